@@ -16,8 +16,10 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libannembed_hip.so")
 MANIFEST = os.path.join(HERE, "build_manifest.json")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+# packed-fp32-ops off: -O3 forms v_pk_{add,mul,fma}_f32 from ordinary float code, and some of their forms have given wrong results now and
+# then; every operation rounds the same either way
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function",
-         "-Wno-unused-result"]
+         "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _sources():
