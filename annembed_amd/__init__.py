@@ -11,10 +11,19 @@ from .api import (DiffusionMaps, DiffusionParams, Embedder, EmbedderParams, Entr
                   KGraphProjection, MatRepr, NodeParams, QualityReport, RangeApprox, RangePrecision, RangeRank, SvdApprox, SvdResult, entropy_optimize,
                   adaptative_range_finder_matrep, quality_estimate_from_edge_length, set_data_box, subspace_iteration, to_proba_edges, transpose_dense_mult_csr, set_summation_order)
 
+
+def __getattr__(name):
+    """points8 works on torch tensors: it is imported when it is first asked for, the rest of the package does without torch"""
+    if name in ("Points8", "teacher_loss", "teacher_grad"):
+        from . import points8
+        return getattr(points8, name)
+    raise AttributeError("module %r has no attribute %r" % (__name__, name))
+
+
 __all__ = [
     "KGraph", "KGraphProjection", "NodeParams", "EmbedderParams", "DiffusionParams", "Embedder", "EntropyOptim",
     "DiffusionMaps", "GraphLaplacian", "MatRepr", "RangeRank", "SvdApprox", "SvdResult", "to_proba_edges", "set_data_box",
     "entropy_optimize", "subspace_iteration", "transpose_dense_mult_csr", "QualityReport", "quality_estimate_from_edge_length", "RangePrecision", "RangeApprox",
     "adaptative_range_finder_matrep",
-    "set_summation_order", "AnnembedError", "load",
+    "set_summation_order", "Points8", "teacher_loss", "teacher_grad", "AnnembedError", "load",
 ]

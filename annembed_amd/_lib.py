@@ -32,6 +32,11 @@ AE_SAMPLER_ROWCDF = 0
 AE_SAMPLER_ALIAS = 1
 AE_PRECISION_F64 = 0
 AE_PRECISION_F32 = 1
+AE_TYPE_F32 = 0
+AE_TYPE_BF16 = 1
+AE_TYPE_F16 = 2
+AE_TEACHER_PROBA = 0
+AE_TEACHER_LOGITS = 1
 
 
 class AnnembedError(RuntimeError):
@@ -167,6 +172,21 @@ SIGNATURES = {
     "ae_embedder_get_cross_entropy": [_vp, _P(_f64), _P(_f64)],
     "ae_quality_estimate_from_edge_length": [_vp, _vp, _u32, _u32, _P(CQualityReport), _vp, _vp],
     "ae_embedder_get_quality_estimate_from_edge_length": [_vp, _u32, _P(CQualityReport), _vp, _vp],
+    "ae_points8_create": [_u64, _u64, _P(_vp)],
+    "ae_points8_destroy": [_vp],
+    "ae_points8_info": [_vp, _P(_u64), _P(_u64), _P(_u64), _P(_u64)],
+    "ae_points8_device": [_vp, _P(_vp), _P(_vp)],
+    "ae_points8_write": [_vp, _vp, _u32, _u64, _u64, _u64, _vp, _vp],
+    "ae_points8_read": [_vp, _u64, _vp, _u64, _vp, _u32, _u64, _vp],
+    "ae_points8_product": [_vp, _u64, _u64, _vp, _u32, _u64, _u64, _vp, _u32, _u64, _vp, _u64, _vp],
+    "ae_points8_product_work": [_vp, _u64, _u64, _P(_u64)],
+    "ae_points8_product_points": [_vp, _u64, _u64, _vp, _u64, _u64, _vp, _u32, _u64, _vp],
+    "ae_points8_product_grad": [_vp, _u64, _u64, _vp, _u32, _u64, _u64, _vp, _u32, _u64, _vp, _u64, _vp],
+    "ae_points8_product_grad_work": [_vp, _u64, _u64, _u32, _P(_u64)],
+    "ae_kgraph_bruteforce_l2_points8": [_vp, _u64, _u64, _u32, _vp, _P(_vp)],
+    "ae_teacher_loss": [_vp, _u32, _u64, _u64, _u64, _vp, _vp, _u32, _u64, _u32, _f32, _vp, _vp, _vp, _vp, _u64, _vp, _u64, _vp],
+    "ae_teacher_loss_work": [_u64, _u64, _P(_u64)],
+    "ae_teacher_grad": [_vp, _u32, _u64, _u64, _u64, _vp, _vp, _vp, _u32, _u64, _u32, _f32, _vp, _vp, _u64, _vp],
 }
 STRING_GETTERS = ["ae_last_error_message", "ae_last_warning_message", "ae_version"]
 

@@ -199,6 +199,16 @@ class KGraph(_Handle):
         return cls._wrap(h)
 
     @classmethod
+    def bruteforce_l2_points8(cls, points, nbng, n=None, first=0):
+        """the exact graph of points first ... first + n - 1 of a Points8 store, as it holds them (ae_kgraph_bruteforce_l2_points8)"""
+        import torch
+        n, first = points._range(n, first)
+        h = C.c_void_p()
+        with torch.cuda.device(points.device):
+            check(L.load().ae_kgraph_bruteforce_l2_points8(points.handle, first, n, nbng, torch.cuda.current_stream().cuda_stream, C.byref(h)))
+        return cls._wrap(h)
+
+    @classmethod
     def bruteforce_l2_grouped(cls, x, nbng, bounds):
         """the exact global kNN graph of points sorted into groups (ae_kgraph_bruteforce_l2_grouped); `.knn_stats` = (fallback rows,
         pairs of the pruned phase, pairs inside the groups)"""

@@ -343,6 +343,29 @@ void bruteforce_knn_rows(const float* d_x, uint64_t n, uint64_t dim, uint32_t k,
                          uint32_t* d_nbr, float* d_dist) {
     bruteforce_knn_rect(d_x, dim, k, nullptr, 0, d_rows, nrows, 0, n, d_nbr, d_dist, false, false, nullptr);
 }
+// exact kNN graph of n >= 2 points on the device, 1 <= nbng < n
+ae_kgraph* kgraph_bruteforce_device(const float* d_x, uint64_t n, uint64_t dim, uint32_t nbng) {
+    std::unique_ptr<ae_kgraph> g(new ae_kgraph);
+    g->n = n;
+    g->max_nbng = nbng;
+    g->nnz = n * nbng;
+    std::vector<uint64_t> indptr(n + 1);
+    for (uint64_t i = 0; i <= n; i++) indptr[i] = i * nbng;
+    g->indptr.alloc(n + 1);
+    g->indptr.upload(indptr.data(), n + 1);
+    g->nbr.alloc(g->nnz);
+    g->dist.alloc(g->nnz);
+    // matrix-core path (knn.hip) for the usual neighbourhood sizes; AE_KNN_LEGACY=1 keeps the plain kernel (A/B)
+    if (nbng + 8 <= 64 && !debug_knob("AE_KNN_LEGACY")) {
+        const uint64_t fell_back = knn_mfma(d_x, n, dim, nbng, g->nbr.p, g->dist.p);
+        if (debug_knob("AE_CE_PROF")) fprintf(stderr, "KNN rows recomputed by the brute-force fallback: %llu of %llu\n",
+                                          (unsigned long long)fell_back, (unsigned long long)n);
+    } else {
+        bruteforce_knn_rows(d_x, n, dim, nbng, nullptr, n, g->nbr.p, g->dist.p);
+    }
+    finish_kgraph(g.get());
+    return g.release();
+}
 }  // namespace ae
 
 extern "C" {
@@ -595,26 +618,7 @@ int32_t ae_kgraph_bruteforce_l2(const float* x, uint64_t n, uint64_t dim, uint32
         DevBuf<float> dx;
         dx.alloc(n * dim);
         dx.upload(x, n * dim);
-        std::unique_ptr<ae_kgraph> g(new ae_kgraph);
-        g->n = n;
-        g->max_nbng = nbng;
-        g->nnz = n * nbng;
-        std::vector<uint64_t> indptr(n + 1);
-        for (uint64_t i = 0; i <= n; i++) indptr[i] = i * nbng;
-        g->indptr.alloc(n + 1);
-        g->indptr.upload(indptr.data(), n + 1);
-        g->nbr.alloc(g->nnz);
-        g->dist.alloc(g->nnz);
-        // matrix-core path (knn.hip) for the usual neighbourhood sizes; AE_KNN_LEGACY=1 keeps the plain kernel (A/B)
-        if (nbng + 8 <= 64 && !debug_knob("AE_KNN_LEGACY")) {
-            const uint64_t fell_back = knn_mfma(dx.p, n, dim, nbng, g->nbr.p, g->dist.p);
-            if (debug_knob("AE_CE_PROF")) fprintf(stderr, "KNN rows recomputed by the brute-force fallback: %llu of %llu\n",
-                                              (unsigned long long)fell_back, (unsigned long long)n);
-        } else {
-            bruteforce_knn_rows(dx.p, n, dim, nbng, nullptr, n, g->nbr.p, g->dist.p);
-        }
-        finish_kgraph(g.get());
-        *out = g.release();
+        *out = kgraph_bruteforce_device(dx.p, n, dim, nbng);
     });
 }
 

@@ -36,5 +36,6 @@ struct Partition {
 void partition_nodes_device(const ae_kgraph* g, const float* d_proba, const float* d_y, uint32_t ydim, uint32_t ystride, uint32_t world, Partition& out);
 void partition_cross_mass_device(const ae_kgraph* g, const float* d_proba, Partition& p);
 ae_kgraph* kgraph_permuted_device(const ae_kgraph* g, const uint32_t* d_order, const uint32_t* d_perm, const float* d_extra, DevBuf<float>* extra2);
+ae_kgraph* kgraph_bruteforce_device(const float* d_x, uint64_t n, uint64_t dim, uint32_t nbng);   // points on the device (core.hip)
 void permute_rows_device(const float* d_src, float* d_dst, uint64_t n, uint32_t dim, const uint32_t* d_order, bool back);
 }  // namespace ae

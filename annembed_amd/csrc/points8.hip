@@ -1,0 +1,308 @@
+// points8.hip -- the store of points in 8 bits: rows quantised as they are written, read back as the values they stand for.
+//
+// Both directions move n dim (1 + size of x) bytes and compute next to nothing: they are bound by HBM, the smallest calls by the launch.
+// A group of 16 lanes owns a block of 128 coordinates (8 a lane: 16 or 32 bytes of x, 8 bytes of codes, whatever the type), so the block's
+// largest magnitude is four DPP rotations within a row of the wave, no LDS and no barrier; a wave covers 4 blocks = 1 or 2 KB of
+// consecutive x.  Blocks are numbered through the whole call (block u = row u / blocks), so rows of any length fill the waves alike.
+#include "points8.h"
+
+using namespace ae;
+
+namespace {
+
+constexpr int kGroups = 16;    // blocks per workgroup and trip
+constexpr int kTrips = 4;      // blocks a group has in flight: 64 to 128 bytes of loads per lane
+constexpr uint32_t kScan = 1024;   // up to this many slots a row looks for a later occurrence of its slot itself
+
+struct Blocks {   // the call's blocks
+    uint64_t units, n;
+    uint32_t nb;
+};
+// row and block of unit `u0 + t`; u0 is the workgroup's first unit
+struct Cursor {
+    uint64_t row0;
+    uint32_t rem0;
+    __device__ Cursor(uint64_t u0, uint32_t nb) {
+        if (u0 >> 32) { row0 = u0 / nb; rem0 = (uint32_t)(u0 - row0 * nb); }
+        else { row0 = (uint32_t)u0 / nb; rem0 = (uint32_t)u0 - (uint32_t)row0 * nb; }
+    }
+    __device__ __forceinline__ void at(uint32_t t, uint32_t nb, uint64_t& row, uint32_t& b) const {
+        const uint32_t x = rem0 + t, q = x / nb;
+        row = row0 + q;
+        b = x - q * nb;
+    }
+};
+
+// the later of two rows with the same slot is the one that is held: every row of the call claims its slot, the largest row wins
+__global__ void __launch_bounds__(256) points8_claim_kernel(const uint32_t* __restrict__ slots, uint32_t n, uint64_t capacity, uint32_t* __restrict__ owner) {
+    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+    if (i >= n) return;
+    const uint32_t s = slots[i];
+    if (s < capacity) atomicMax(&owner[s], i + 1);
+}
+__global__ void __launch_bounds__(256) points8_release_kernel(const uint32_t* __restrict__ slots, uint32_t n, uint64_t capacity, uint32_t* __restrict__ owner) {
+    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+    if (i >= n) return;
+    const uint32_t s = slots[i];
+    if (s < capacity) owner[s] = 0;
+}
+
+// SLOTS 0: row i to first + i.  1: to slots[i], each row scans for a later row of the same slot.  2: to slots[i] where owner says so.
+template <int TYPE, bool VEC, int SLOTS>
+__global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<TYPE>::T* __restrict__ x, uint64_t ldx, uint64_t dim, Blocks bl, uint64_t first,
+                                                            const uint32_t* __restrict__ slots, const uint32_t* __restrict__ owner, uint64_t capacity,
+                                                            uint8_t* __restrict__ codes, uint64_t row_bytes, uint8_t* __restrict__ scales, uint32_t scale_stride) {
+    const uint64_t u0 = blockIdx.x * (uint64_t)(kGroups * kTrips);
+    const Cursor cur(u0, bl.nb);
+    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
+    float v[kTrips][8];
+    uint64_t row[kTrips];
+    uint32_t b[kTrips];
+    bool live[kTrips];
+#pragma unroll
+    for (int t = 0; t < kTrips; t++) {
+        const uint32_t off = t * kGroups + group;
+        cur.at(off, bl.nb, row[t], b[t]);
+        live[t] = u0 + off < bl.units;
+        const uint64_t k = b[t] * (uint64_t)kBlock + lane * 8;
+        const int count = !live[t] || k >= dim ? 0 : (int)min((uint64_t)8, dim - k);
+        load8<TYPE>(x + (count ? row[t] * ldx + k : 0), VEC && count == 8, count, v[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < kTrips; t++) {
+        const uint32_t byte = scale_byte(max16(amax8(v[t])));
+        uint64_t to = first + row[t];
+        if constexpr (SLOTS != 0) {
+            if (live[t]) {
+                const uint32_t s = slots[row[t]];
+                to = s;
+                live[t] = s < capacity;
+                if constexpr (SLOTS == 2) live[t] = live[t] && owner[s] == (uint32_t)row[t] + 1;
+            }
+            if constexpr (SLOTS == 1) {
+                bool later = false;
+                if (live[t])
+                    for (uint64_t j = row[t] + 1 + lane; j < bl.n; j += 16) later |= slots[j] == (uint32_t)to;
+                const uint64_t seen = __ballot(later);
+                live[t] = live[t] && ((seen >> (threadIdx.x & 48)) & 0xFFFFull) == 0;
+            }
+        }
+        const uint64_t k = b[t] * (uint64_t)kBlock + lane * 8;
+        if (live[t] && k < row_bytes) *reinterpret_cast<uint2*>(codes + to * row_bytes + k) = encode8(v[t], byte);
+        if (live[t] && lane == 0) scales[to * scale_stride + b[t]] = (uint8_t)byte;
+    }
+}
+
+template <int TYPE, bool VEC, bool SLOTS>
+__global__ void __launch_bounds__(256) points8_read_kernel(const uint8_t* __restrict__ codes, uint64_t row_bytes, const uint8_t* __restrict__ scales, uint32_t scale_stride,
+                                                           uint64_t capacity, uint64_t first, const uint32_t* __restrict__ slots, Blocks bl,
+                                                           typename Elem<TYPE>::T* __restrict__ x, uint64_t ldx, uint64_t dim) {
+    const uint64_t u0 = blockIdx.x * (uint64_t)(kGroups * kTrips);
+    const Cursor cur(u0, bl.nb);
+    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
+    uint2 c[kTrips];
+    uint32_t byte[kTrips];
+    uint64_t row[kTrips];
+    uint32_t b[kTrips];
+    int count[kTrips];
+    bool bad[kTrips];
+#pragma unroll
+    for (int t = 0; t < kTrips; t++) {
+        const uint32_t off = t * kGroups + group;
+        cur.at(off, bl.nb, row[t], b[t]);
+        const uint64_t k = b[t] * (uint64_t)kBlock + lane * 8;
+        count[t] = u0 + off >= bl.units || k >= dim ? 0 : (int)min((uint64_t)8, dim - k);
+        c[t] = make_uint2(0, 0);
+        byte[t] = 0;
+        bad[t] = false;
+        if (count[t]) {
+            uint64_t from = first + row[t];
+            if constexpr (SLOTS) {
+                from = slots[row[t]];
+                bad[t] = from >= capacity && from != 0xFFFFFFFFull;
+            }
+            if (from < capacity) {
+                c[t] = *reinterpret_cast<const uint2*>(codes + from * row_bytes + k);
+                byte[t] = scales[from * scale_stride + b[t]];
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kTrips; t++) {
+        float v[8];
+        decode8(c[t], byte[t], v);
+        if (SLOTS && bad[t]) {
+#pragma unroll
+            for (int q = 0; q < 8; q++) v[q] = __uint_as_float(0x7FC00000u);
+        }
+        const uint64_t k = b[t] * (uint64_t)kBlock + lane * 8;
+        if (count[t]) store8<TYPE>(x + row[t] * ldx + k, VEC && count[t] == 8, count[t], v);
+    }
+}
+
+Blocks blocks_of(uint64_t n, uint64_t dim) {
+    Blocks bl;
+    bl.n = n;
+    bl.nb = points8_blocks(dim);
+    bl.units = n * bl.nb;
+    return bl;
+}
+unsigned trips_grid(const Blocks& bl) {
+    const uint64_t g = (bl.units + kGroups * kTrips - 1) / (kGroups * kTrips);
+    if (g * 256 > 0xFFFFFFFFull) fail(AE_ERR_INVALID_ARG, "%llu rows of %u blocks are more than one call takes", (unsigned long long)bl.n, bl.nb);
+    return (unsigned)g;
+}
+
+template <int SLOTS>
+void launch_write(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint64_t first, const uint32_t* slots, const uint32_t* owner, uint64_t capacity,
+                  uint8_t* codes, uint8_t* scales, hipStream_t s) {
+    const Blocks bl = blocks_of(n, dim);
+    const unsigned grid = trips_grid(bl);
+    by_type(type, [&](auto ty) {
+        constexpr int TYPE = decltype(ty)::value;
+        const auto* x = static_cast<const typename Elem<TYPE>::T*>(d_x);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales, points8_scale_stride(dim));
+        };
+        if (vector_rows(d_x, type, ldx)) go(points8_write_kernel<TYPE, true, SLOTS>);
+        else go(points8_write_kernel<TYPE, false, SLOTS>);
+    });
+    check_launch("points8_write");
+}
+
+void read_rows(const ae_points8* p, uint64_t first, const uint32_t* slots, uint64_t n, void* d_x, uint32_t type, uint64_t ldx, hipStream_t s) {
+    const Blocks bl = blocks_of(n, p->dim);
+    const unsigned grid = trips_grid(bl);
+    by_type(type, [&](auto ty) {
+        constexpr int TYPE = decltype(ty)::value;
+        auto* x = static_cast<typename Elem<TYPE>::T*>(d_x);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, (const uint8_t*)p->codes.p, p->row_bytes, (const uint8_t*)p->scales.p, p->scale_stride, p->capacity, first,
+                               slots, bl, x, ldx, p->dim);
+        };
+        const bool vec = vector_rows(d_x, type, ldx);
+        if (slots) { if (vec) go(points8_read_kernel<TYPE, true, true>); else go(points8_read_kernel<TYPE, false, true>); }
+        else { if (vec) go(points8_read_kernel<TYPE, true, false>); else go(points8_read_kernel<TYPE, false, false>); }
+    });
+    check_launch("points8_read");
+}
+
+}  // namespace
+
+namespace ae {
+
+void check_points8(const ae_points8* p, uint64_t first, uint64_t n, const char* what) {
+    if (!p) fail(AE_ERR_INVALID_ARG, "%s: the store is NULL", what);
+    int dev = 0;
+    AE_HIP(hipGetDevice(&dev));
+    if (dev != p->device) fail(AE_ERR_INVALID_ARG, "%s: the store lives on device %d, the current device is %d", what, p->device, dev);
+    if (first > p->capacity || n > p->capacity - first)
+        fail(AE_ERR_INVALID_ARG, "%s: rows %llu ... + %llu are outside a store of %llu", what, (unsigned long long)first, (unsigned long long)n, (unsigned long long)p->capacity);
+}
+
+void points8_quantise(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint8_t* codes, uint8_t* scales, hipStream_t s) {
+    launch_write<0>(d_x, type, n, ldx, dim, 0, nullptr, nullptr, n, codes, scales, s);
+}
+
+}  // namespace ae
+
+extern "C" {
+
+int32_t ae_points8_create(uint64_t capacity, uint64_t dim, ae_points8** out) {
+    return guard([&] {
+        require_device();
+        if (!out) fail(AE_ERR_INVALID_ARG, "ae_points8_create: out is NULL");
+        if (capacity == 0 || capacity >= 0xFFFFFFFFull) fail(AE_ERR_INVALID_ARG, "ae_points8_create: a capacity of %llu rows is out of range", (unsigned long long)capacity);
+        if (dim == 0 || dim > (1u << 20)) fail(AE_ERR_INVALID_ARG, "ae_points8_create: dim %llu is not in [1, 2^20]", (unsigned long long)dim);
+        std::unique_ptr<ae_points8> p(new ae_points8);
+        p->capacity = capacity;
+        p->dim = dim;
+        p->row_bytes = points8_row_bytes(dim);
+        p->blocks = points8_blocks(dim);
+        p->scale_stride = points8_scale_stride(dim);
+        AE_HIP(hipGetDevice(&p->device));
+        p->codes.alloc(capacity * p->row_bytes);
+        p->scales.alloc(capacity * p->scale_stride);
+        p->owner.alloc(capacity);
+        p->codes.zero();
+        p->scales.zero();
+        p->owner.zero();
+        sync();
+        *out = p.release();
+    });
+}
+int32_t ae_points8_destroy(ae_points8* p) {
+    return guard([&] { delete p; });
+}
+int32_t ae_points8_info(const ae_points8* p, uint64_t* capacity, uint64_t* dim, uint64_t* row_bytes, uint64_t* scale_stride) {
+    return guard([&] {
+        if (!p) fail(AE_ERR_INVALID_ARG, "ae_points8_info: the store is NULL");
+        if (capacity) *capacity = p->capacity;
+        if (dim) *dim = p->dim;
+        if (row_bytes) *row_bytes = p->row_bytes;
+        if (scale_stride) *scale_stride = p->scale_stride;
+    });
+}
+int32_t ae_points8_device(const ae_points8* p, void** d_codes, void** d_scales) {
+    return guard([&] {
+        if (!p || !d_codes || !d_scales) fail(AE_ERR_INVALID_ARG, "ae_points8_device: null argument");
+        *d_codes = p->codes.p;
+        *d_scales = p->scales.p;
+    });
+}
+
+int32_t ae_points8_write(ae_points8* p, const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t first, const uint32_t* d_slots, void* stream) {
+    return guard([&] {
+        require_device();
+        check_points8(p, d_slots ? 0 : first, d_slots ? 0 : n, "ae_points8_write");
+        check_type(type, "ae_points8_write");
+        if (n == 0) return;
+        check_rows(d_x, type, n, p->dim, ldx, "ae_points8_write: x");
+        hipStream_t s = (hipStream_t)stream;
+        if (!d_slots) {
+            launch_write<0>(d_x, type, n, ldx, p->dim, first, nullptr, nullptr, p->capacity, p->codes.p, p->scales.p, s);
+            return;
+        }
+        check_aligned(d_slots, 4, "ae_points8_write: slots");
+        if (n > 0x7FFFFFFFull) fail(AE_ERR_INVALID_ARG, "ae_points8_write: %llu slots are more than one call takes", (unsigned long long)n);
+        // The last row of a repeated slot is held.  Few rows: every block scans the slots behind its own, one launch.  More: the rows claim
+        // their slots first and give them back afterwards, three launches.
+        if (n <= kScan) {
+            launch_write<1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, s);
+            return;
+        }
+        const unsigned grid = blocks_for(n, 256);
+        hipLaunchKernelGGL(points8_claim_kernel, dim3(grid), dim3(256), 0, s, d_slots, (uint32_t)n, p->capacity, p->owner.p);
+        check_launch("points8_claim");
+        launch_write<2>(d_x, type, n, ldx, p->dim, 0, d_slots, p->owner.p, p->capacity, p->codes.p, p->scales.p, s);
+        hipLaunchKernelGGL(points8_release_kernel, dim3(grid), dim3(256), 0, s, d_slots, (uint32_t)n, p->capacity, p->owner.p);
+        check_launch("points8_release");
+    });
+}
+
+int32_t ae_points8_read(const ae_points8* p, uint64_t first, const uint32_t* d_slots, uint64_t n, void* d_x, uint32_t type, uint64_t ldx, void* stream) {
+    return guard([&] {
+        require_device();
+        check_points8(p, d_slots ? 0 : first, d_slots ? 0 : n, "ae_points8_read");
+        check_type(type, "ae_points8_read");
+        if (n == 0) return;
+        check_rows(d_x, type, n, p->dim, ldx, "ae_points8_read: x");
+        if (d_slots) check_aligned(d_slots, 4, "ae_points8_read: slots");
+        read_rows(p, first, d_slots, n, d_x, type, ldx, (hipStream_t)stream);
+    });
+}
+
+int32_t ae_kgraph_bruteforce_l2_points8(const ae_points8* p, uint64_t first, uint64_t n, uint32_t nbng, void* stream, ae_kgraph** out) {
+    return guard([&] {
+        require_device();
+        check_points8(p, first, n, "ae_kgraph_bruteforce_l2_points8");
+        if (!out || n < 2 || nbng == 0 || nbng >= n) fail(AE_ERR_INVALID_ARG, "ae_kgraph_bruteforce_l2_points8: bad arguments");
+        DevBuf<float> dx;
+        dx.alloc(n * p->dim);
+        AE_HIP(hipStreamSynchronize((hipStream_t)stream));
+        read_rows(p, first, nullptr, n, dx.p, AE_TYPE_F32, p->dim, ae::stream());
+        *out = kgraph_bruteforce_device(dx.p, n, p->dim, nbng);
+    });
+}
+
+}  // extern "C"

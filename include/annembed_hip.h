@@ -588,6 +588,85 @@ int32_t ae_embedder_get_quality_estimate_from_edge_length(const ae_embedder *e, 
                                                           ae_quality_report *rep,
                                                           double *ratio_by_node, double *first_dist);
 
+/* ------------------------------------------------------------------------------------------------
+ * Points held in 8 bits, the product of rows with them, and the teacher's loss (no reference counterpart: what a user who trains an
+ * encoder against the graph's edge probabilities needs beside the graph).
+ *
+ * These calls take device memory of the CURRENT device and a hipStream_t (`stream`; NULL is the device's default stream, as for
+ * HIP itself): they check their arguments, launch on that stream and return -- no synchronisation, no allocation, nothing kept between
+ * calls, so they may be captured into a graph.  Scratch memory is the caller's: the *_work functions say how many bytes a call of
+ * that size needs (0: d_work may be NULL); it has to be 16-byte aligned and two calls that may run at the same time need scratch of their own.
+ * Rows are row-major with a stride of ld* ELEMENTS (>= the row's length; rows of an even 16 bytes are read fastest, any alignment of an
+ * element's size works).  n, m, rows = 0 is a call that does nothing.
+ *
+ * Format: a row of `dim` coordinates in blocks of 128 (the last may be shorter).  a = the largest magnitude among the finite values of the
+ * block, e = the smallest integer >= -126 with a <= 448 * 2^e.  A coordinate is the e4m3 number nearest to x * 2^-e (ties to even); NaN
+ * and the infinities are held as NaN.  The scale byte of the block is e + 127.  The value held is code * 2^e.  The scale is a power of two
+ * because that costs an 8-bit float none of its relative precision (2^-4), makes x * 2^-e exact (the codes do not depend on how the
+ * division is done), makes the value held exact in bf16, and is the scale that the matrix cores multiply by themselves.
+ * ------------------------------------------------------------------------------------------------ */
+enum { AE_TYPE_F32 = 0, AE_TYPE_BF16 = 1, AE_TYPE_F16 = 2 };
+typedef struct ae_points8 ae_points8;
+/* room for `capacity` rows (< 2^32 - 1) of `dim` coordinates (1 ... 2^20) on the current device, all of them zero.  Synchronous. */
+int32_t ae_points8_create(uint64_t capacity, uint64_t dim, ae_points8 **out);
+int32_t ae_points8_destroy(ae_points8 *p);
+/* row_bytes: bytes from row to row of the codes (dim rounded up to 16); scale_stride: from row to row of the scale bytes */
+int32_t ae_points8_info(const ae_points8 *p, uint64_t *capacity, uint64_t *dim, uint64_t *row_bytes, uint64_t *scale_stride);
+/* the device memory itself: codes[capacity][row_bytes], scales[capacity][scale_stride] */
+int32_t ae_points8_device(const ae_points8 *p, void **d_codes, void **d_scales);
+/* Row i of x (n rows of dim values) goes to row d_slots[i] of the store, or to row first + i where d_slots is NULL.  A slot outside the
+   store (0xFFFFFFFF marks padding) is skipped; where a slot comes several times the LAST of its rows is held.  Other rows stay as they are.
+   Two writes of one store must not run at the same time. */
+int32_t ae_points8_write(ae_points8 *p, const void *d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t first,
+                         const uint32_t *d_slots, void *stream);
+/* The values of rows first ... first + n - 1, or d_slots[0 ... n - 1], rounded to `type` (exact in f32 and bf16 within their ranges).  Slot
+   0xFFFFFFFF reads as zeros, any other slot outside the store as NaN. */
+int32_t ae_points8_read(const ae_points8 *p, uint64_t first, const uint32_t *d_slots, uint64_t n, void *d_x, uint32_t type,
+                        uint64_t ldx, void *stream);
+/* c[i][j] = <q(x_i), p_{first + j}>, i < m, j < n: the rows x quantised as ae_points8_write would, times the values held, rounded once to
+   `ctype`.  c of f32: exact products, f32 sums.  c of 16 bits: the 8-bit matrix cores, whose sums of eight consecutive products keep 13 bits below
+   the largest of them -- at most 7 * 2^-13 (in the root mean square about 1e-5) of sum_k |x_k p_k|, beside the rounding to 16 bits.  A NaN
+   coordinate makes its products NaN. */
+int32_t ae_points8_product(const ae_points8 *p, uint64_t first, uint64_t n, const void *d_x, uint32_t xtype, uint64_t m, uint64_t ldx,
+                           void *d_c, uint32_t ctype, uint64_t ldc, void *d_work, uint64_t work_bytes, void *stream);
+int32_t ae_points8_product_work(const ae_points8 *p, uint64_t n, uint64_t m, uint64_t *bytes);
+/* the same for rows q_first ... q_first + m - 1 of another (or the same) store of equal dim */
+int32_t ae_points8_product_points(const ae_points8 *p, uint64_t first, uint64_t n, const ae_points8 *q, uint64_t q_first, uint64_t m,
+                                  void *d_c, uint32_t ctype, uint64_t ldc, void *stream);
+/* The gradient of ae_points8_product to its rows, q taken as the identity: dx[i][k] = sum_j dc[i][j] * p_{first + j}[k].  dc enters exactly
+   whatever its type (but for what lies below 2^-126), sums are f32 in an order that depends on the sizes only. */
+int32_t ae_points8_product_grad(const ae_points8 *p, uint64_t first, uint64_t n, const void *d_dc, uint32_t dctype, uint64_t m,
+                                uint64_t lddc, void *d_dx, uint32_t xtype, uint64_t lddx, void *d_work, uint64_t work_bytes, void *stream);
+int32_t ae_points8_product_grad_work(const ae_points8 *p, uint64_t n, uint64_t m, uint32_t dctype, uint64_t *bytes);
+/* ae_kgraph_bruteforce_l2 of the values held in rows first ... first + n - 1: exact neighbours and distances of the points as the store has
+   them (they are read back in f32 on the device, never through the host).  Waits for `stream`, where the rows were written. */
+int32_t ae_kgraph_bruteforce_l2_points8(const ae_points8 *p, uint64_t first, uint64_t n, uint32_t nbng, void *stream, ae_kgraph **out);
+
+/* Cross entropy of rows of logits against a teacher's top list, relative to the teacher's own entropy (a Kullback-Leibler divergence
+   where the list's probabilities sum to 1).  Row r has the logits s_v, v < cols, and a list of k entries (1 ... 1024): d_idx[r * ldk + j] names a
+   column, 0xFFFFFFFF an empty place, and d_list[r * ldk + j] is
+     AE_TEACHER_PROBA   the teacher's probability p_j, as ae_node_params_get has it for a graph row (taken as given: sums below 1 are a
+                        truncated list),
+     AE_TEACHER_LOGITS  the teacher's logit t_j: p = softmax(t / temperature) over the row's list (-inf: p = 0).
+   With ln q = ln softmax(s / temperature):   loss_r = w_r sum_j p_j (ln p_j - ln q_{idx_j}),   w_r = d_row_weight[r] (NULL: 1)
+                                               d loss_r / d s_v = w_r (q_v sum_j p_j - sum_{j: idx_j = v} p_j) / temperature.
+   A column may come several times in a list: its probabilities add up.  p_j = 0 contributes nothing; p_j > 0 on a logit of -inf makes the
+   loss +inf.  A row of weight 0 is not looked at (its logits and list may hold anything): loss 0, gradient 0; so are rows whose logits
+   are all -inf.  A column index >= cols, a NaN or a +inf among a row's logits makes that row NaN.
+   d_loss[rows] f32; d_stats[rows][2] f32: (the largest logit, ln sum_v exp((s_v - largest) / temperature)), (-inf, 0) for rows left out --
+   what ae_teacher_grad needs.  d_grad (NULL: not wanted): the gradient of sum_r loss_r in the logits' type, in the same pass; it may be
+   d_logits itself (ldg = ld). */
+enum { AE_TEACHER_PROBA = 0, AE_TEACHER_LOGITS = 1 };
+int32_t ae_teacher_loss(const void *d_logits, uint32_t type, uint64_t rows, uint64_t cols, uint64_t ld, const uint32_t *d_idx,
+                        const float *d_list, uint32_t k, uint64_t ldk, uint32_t kind, float temperature, const float *d_row_weight,
+                        float *d_loss, float *d_stats, void *d_grad, uint64_t ldg, void *d_work, uint64_t work_bytes, void *stream);
+int32_t ae_teacher_loss_work(uint64_t rows, uint64_t cols, uint64_t *bytes);
+/* The gradient from the statistics of an earlier ae_teacher_loss on the same logits, under each row's own upstream gradient: w_r above is
+   d_dloss[r] (include the row's weight in it).  d_grad may be d_logits. */
+int32_t ae_teacher_grad(const void *d_logits, uint32_t type, uint64_t rows, uint64_t cols, uint64_t ld, const float *d_stats,
+                        const uint32_t *d_idx, const float *d_list, uint32_t k, uint64_t ldk, uint32_t kind, float temperature,
+                        const float *d_dloss, void *d_grad, uint64_t ldg, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
