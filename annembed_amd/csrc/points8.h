@@ -6,7 +6,7 @@ struct ae_points8 {
     uint64_t capacity = 0, dim = 0;
     uint64_t row_bytes = 0;      // dim rounded up to 16: every row starts on 16 bytes; the bytes beyond dim stay 0
     uint32_t blocks = 0;         // ceil(dim / 128)
-    uint32_t scale_stride = 0;   // blocks rounded up to 4: the matrix cores' scale operand takes four blocks as one dword
+    uint64_t scale_stride = 0;   // scales[block][row]: from block to block; the rows of a block lie together, as the matrix cores take them
     int device = 0;
     ae::DevBuf<uint8_t> codes, scales;
     ae::DevBuf<uint32_t> owner;  // per row: which row of the running write holds it (0 between writes)
@@ -20,13 +20,16 @@ struct Rows8 {   // rows of codes with their scales: part of a store, or quantis
     const uint8_t* codes;
     const uint8_t* scales;
     uint64_t row_bytes;
-    uint32_t scale_stride;
+    uint64_t scale_stride;
     uint64_t rows;
 };
 
 inline uint64_t points8_row_bytes(uint64_t dim) { return (dim + 15) / 16 * 16; }
 inline uint32_t points8_blocks(uint64_t dim) { return (uint32_t)((dim + kBlock - 1) / kBlock); }
-inline uint32_t points8_scale_stride(uint64_t dim) { return (points8_blocks(dim) + 3) / 4 * 4; }
+// bytes from block to block of the scales of `rows` rows, and what lies behind the last one: a tile takes the bytes of rows that do not exist
+// along (they multiply zeros, and no result of theirs is written)
+inline uint64_t points8_scale_stride(uint64_t rows) { return (rows + 15) / 16 * 16; }
+constexpr uint64_t kScaleSlack = 512;
 inline uint64_t type_size(uint32_t type) { return type == AE_TYPE_F32 ? 4 : 2; }
 inline void check_type(uint32_t type, const char* what) {
     if (type > AE_TYPE_F16) fail(AE_ERR_INVALID_ARG, "%s: unknown element type %u (AE_TYPE_F32, AE_TYPE_BF16, AE_TYPE_F16)", what, type);
@@ -44,10 +47,10 @@ inline void check_rows(const void* ptr, uint32_t type, uint64_t rows, uint64_t l
 }
 void check_points8(const ae_points8* p, uint64_t first, uint64_t n, const char* what);   // on the current device, rows in range
 inline Rows8 points8_rows(const ae_points8* p, uint64_t first, uint64_t n) {
-    return Rows8{p->codes.p + first * p->row_bytes, p->scales.p + first * p->scale_stride, p->row_bytes, p->scale_stride, n};
+    return Rows8{p->codes.p + first * p->row_bytes, p->scales.p + first, p->row_bytes, p->scale_stride, n};
 }
-// n rows of x into codes / scales (rows of the layout above), row i to row first + i
-void points8_quantise(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint8_t* codes, uint8_t* scales, hipStream_t s);
+// n rows of x into codes[n][row_bytes] / scales[blocks][scale_stride]
+void points8_quantise(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint8_t* codes, uint8_t* scales, uint64_t scale_stride, hipStream_t s);
 
 // can rows at ptr with this stride be accessed 16 bytes at a time?
 inline bool vector_rows(const void* ptr, uint32_t type, uint64_t ld) { return (uintptr_t)ptr % 16 == 0 && ld * type_size(type) % 16 == 0; }

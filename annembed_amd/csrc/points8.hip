@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(256) points8_release_kernel(const uint32_t* __
 template <int TYPE, bool VEC, int SLOTS>
 __global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<TYPE>::T* __restrict__ x, uint64_t ldx, uint64_t dim, Blocks bl, uint64_t first,
                                                             const uint32_t* __restrict__ slots, const uint32_t* __restrict__ owner, uint64_t capacity,
-                                                            uint8_t* __restrict__ codes, uint64_t row_bytes, uint8_t* __restrict__ scales, uint32_t scale_stride) {
+                                                            uint8_t* __restrict__ codes, uint64_t row_bytes, uint8_t* __restrict__ scales, uint64_t scale_stride) {
     const uint64_t u0 = blockIdx.x * (uint64_t)(kGroups * kTrips);
     const Cursor cur(u0, bl.nb);
     const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
@@ -89,12 +89,12 @@ __global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<
         }
         const uint64_t k = b[t] * (uint64_t)kBlock + lane * 8;
         if (live[t] && k < row_bytes) *reinterpret_cast<uint2*>(codes + to * row_bytes + k) = encode8(v[t], byte);
-        if (live[t] && lane == 0) scales[to * scale_stride + b[t]] = (uint8_t)byte;
+        if (live[t] && lane == 0) scales[b[t] * scale_stride + to] = (uint8_t)byte;
     }
 }
 
 template <int TYPE, bool VEC, bool SLOTS>
-__global__ void __launch_bounds__(256) points8_read_kernel(const uint8_t* __restrict__ codes, uint64_t row_bytes, const uint8_t* __restrict__ scales, uint32_t scale_stride,
+__global__ void __launch_bounds__(256) points8_read_kernel(const uint8_t* __restrict__ codes, uint64_t row_bytes, const uint8_t* __restrict__ scales, uint64_t scale_stride,
                                                            uint64_t capacity, uint64_t first, const uint32_t* __restrict__ slots, Blocks bl,
                                                            typename Elem<TYPE>::T* __restrict__ x, uint64_t ldx, uint64_t dim) {
     const uint64_t u0 = blockIdx.x * (uint64_t)(kGroups * kTrips);
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(256) points8_read_kernel(const uint8_t* __rest
             }
             if (from < capacity) {
                 c[t] = *reinterpret_cast<const uint2*>(codes + from * row_bytes + k);
-                byte[t] = scales[from * scale_stride + b[t]];
+                byte[t] = scales[b[t] * scale_stride + from];
             }
         }
     }
@@ -155,14 +155,14 @@ unsigned trips_grid(const Blocks& bl) {
 
 template <int SLOTS>
 void launch_write(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint64_t first, const uint32_t* slots, const uint32_t* owner, uint64_t capacity,
-                  uint8_t* codes, uint8_t* scales, hipStream_t s) {
+                  uint8_t* codes, uint8_t* scales, uint64_t scale_stride, hipStream_t s) {
     const Blocks bl = blocks_of(n, dim);
     const unsigned grid = trips_grid(bl);
     by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         const auto* x = static_cast<const typename Elem<TYPE>::T*>(d_x);
         auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales, points8_scale_stride(dim));
+            hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales, scale_stride);
         };
         if (vector_rows(d_x, type, ldx)) go(points8_write_kernel<TYPE, true, SLOTS>);
         else go(points8_write_kernel<TYPE, false, SLOTS>);
@@ -200,8 +200,8 @@ void check_points8(const ae_points8* p, uint64_t first, uint64_t n, const char* 
         fail(AE_ERR_INVALID_ARG, "%s: rows %llu ... + %llu are outside a store of %llu", what, (unsigned long long)first, (unsigned long long)n, (unsigned long long)p->capacity);
 }
 
-void points8_quantise(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint8_t* codes, uint8_t* scales, hipStream_t s) {
-    launch_write<0>(d_x, type, n, ldx, dim, 0, nullptr, nullptr, n, codes, scales, s);
+void points8_quantise(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint8_t* codes, uint8_t* scales, uint64_t scale_stride, hipStream_t s) {
+    launch_write<0>(d_x, type, n, ldx, dim, 0, nullptr, nullptr, n, codes, scales, scale_stride, s);
 }
 
 }  // namespace ae
@@ -219,10 +219,10 @@ int32_t ae_points8_create(uint64_t capacity, uint64_t dim, ae_points8** out) {
         p->dim = dim;
         p->row_bytes = points8_row_bytes(dim);
         p->blocks = points8_blocks(dim);
-        p->scale_stride = points8_scale_stride(dim);
+        p->scale_stride = points8_scale_stride(capacity);
         AE_HIP(hipGetDevice(&p->device));
         p->codes.alloc(capacity * p->row_bytes);
-        p->scales.alloc(capacity * p->scale_stride);
+        p->scales.alloc(p->blocks * p->scale_stride + kScaleSlack);
         p->owner.alloc(capacity);
         p->codes.zero();
         p->scales.zero();
@@ -260,7 +260,7 @@ int32_t ae_points8_write(ae_points8* p, const void* d_x, uint32_t type, uint64_t
         check_rows(d_x, type, n, p->dim, ldx, "ae_points8_write: x");
         hipStream_t s = (hipStream_t)stream;
         if (!d_slots) {
-            launch_write<0>(d_x, type, n, ldx, p->dim, first, nullptr, nullptr, p->capacity, p->codes.p, p->scales.p, s);
+            launch_write<0>(d_x, type, n, ldx, p->dim, first, nullptr, nullptr, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
             return;
         }
         check_aligned(d_slots, 4, "ae_points8_write: slots");
@@ -268,13 +268,13 @@ int32_t ae_points8_write(ae_points8* p, const void* d_x, uint32_t type, uint64_t
         // The last row of a repeated slot is held.  Few rows: every block scans the slots behind its own, one launch.  More: the rows claim
         // their slots first and give them back afterwards, three launches.
         if (n <= kScan) {
-            launch_write<1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, s);
+            launch_write<1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
             return;
         }
         const unsigned grid = blocks_for(n, 256);
         hipLaunchKernelGGL(points8_claim_kernel, dim3(grid), dim3(256), 0, s, d_slots, (uint32_t)n, p->capacity, p->owner.p);
         check_launch("points8_claim");
-        launch_write<2>(d_x, type, n, ldx, p->dim, 0, d_slots, p->owner.p, p->capacity, p->codes.p, p->scales.p, s);
+        launch_write<2>(d_x, type, n, ldx, p->dim, 0, d_slots, p->owner.p, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
         hipLaunchKernelGGL(points8_release_kernel, dim3(grid), dim3(256), 0, s, d_slots, (uint32_t)n, p->capacity, p->owner.p);
         check_launch("points8_release");
     });

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) grad_tile_kernel(GradArgs a, uint32_t til
             const uint64_t j = j0 + jg * 8 + e, k = k0 + kg * 4;
             const bool in = j < je && k < a.p.row_bytes;
             code[e] = in ? *reinterpret_cast<const uint32_t*>(a.p.codes + j * a.p.row_bytes + k) : 0;
-            byte[e] = in ? a.p.scales[j * a.p.scale_stride + tk] : 0;
+            byte[e] = in ? a.p.scales[tk * a.p.scale_stride + j] : 0;
         }
     };
     f32x16 acc[2][2];

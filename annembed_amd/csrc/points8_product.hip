@@ -1,8 +1,8 @@
 // points8_product.hip -- rows times the points held in 8 bits: c[i][j] = <x_i, p_j> on the scaled 8-bit matrix cores.
 //
-// v_mfma_scale_f32_32x32x64_f8f6f4 takes 32 + 32 rows of 64 e4m3 codes and one power-of-two scale per row and 32 coordinates: two of them
-// cover a block of 128 with the block's own scale bytes, so the scales cost no arithmetic at all.  Which of the 64 coordinates a lane holds
-// does not matter as long as both operands agree (the scale is one for the block).
+// v_mfma_scale_f32_16x16x128_f8f6f4 takes 16 + 16 rows of 128 e4m3 codes with a power-of-two scale per row and 32 coordinates: a block with its
+// own scale byte, so the scales cost no arithmetic at all.  Which of the 128 coordinates a lane holds does not matter as long as both
+// operands agree.  (The 32 x 32 x 64 form does the same work for more power: 3.5 against 4.0 PFLOP/s on random codes, nothing but products.)
 //
 // The 8-bit cores add eight products of consecutive codes at a time, cut 13 bits below the largest of the eight (measured on this chip:
 // 2^12 + 2^-1 is kept, 2^12 + 2^-2 is 2^12).  That is at most 7 * 2^-13 of the sum of the products' magnitudes, 1e-5 of it in the
@@ -14,13 +14,29 @@ using namespace ae;
 
 namespace {
 
-// Tiles in LDS: a row's block of 128 codes is 8 chunks of 16 bytes; chunk c of row r lies at place c ^ ((r >> 1) & 7), so 16 lanes that read
-// the same chunk of consecutive rows touch all 64 banks once.  The copy to LDS writes lane after lane, so the lanes permute what they fetch.
-__device__ __forceinline__ int swizzled(int row, int chunk) { return row * kBlock + ((chunk ^ ((row >> 1) & 7)) << 4); }
-
-
 __device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b) {
     return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+}
+// the scale byte of row i of the FM (FN) that a lane holds, four of them in a dword
+__device__ __forceinline__ uint32_t byte_of(const uint32_t* dwords, int i) { return (dwords[i >> 2] >> ((i & 3) * 8)) & 255u; }
+
+// lanes 32 ... 63 of a and lanes 0 ... 31 of b change places
+__device__ __forceinline__ void swap32(u32x4& a, u32x4& b) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const auto r = __builtin_amdgcn_permlane32_swap(a[e], b[e], false, false);
+        a[e] = r[0];
+        b[e] = r[1];
+    }
+}
+// the odd groups of 16 lanes of a and the even ones of b
+__device__ __forceinline__ void swap16(u32x4& a, u32x4& b) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const auto r = __builtin_amdgcn_permlane16_swap(a[e], b[e], false, false);
+        a[e] = r[0];
+        b[e] = r[1];
+    }
 }
 
 struct ProductArgs {
@@ -29,190 +45,299 @@ struct ProductArgs {
     void* c;
     uint64_t ldc;
     uint32_t tiles_m, tiles_n;
-    uint32_t vec;     // rows of c can be written 16 bytes at a time
+    uint32_t vec;     // rows of c can be written 16 bytes at a time, and a tile's rows span less than 2 GiB
 };
 
-// Which tile a workgroup owns.  Workgroups go to the 8 XCDs in turn, each with an L2 of its own: the tiles are handed out so that an XCD
-// walks a run of them, kPanel rows of tiles at a time, and the points it fetched serve all rows of the panel.
+// The tiles of a workgroup.  Workgroups go to the 8 XCDs in turn, each with an L2 of its own: an XCD owns a run of the tiles, kPanel rows of
+// tiles at a time, and its workgroups walk it side by side, so that the points one of them fetched serve the panel's other rows.
 constexpr uint32_t kPanel = 4;
-__device__ __forceinline__ void tile_of(uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
-    const uint32_t total = tiles_m * tiles_n, each = total / 8, more = total % 8, xcd = blockIdx.x % 8, at = blockIdx.x / 8;
-    const uint32_t id = xcd * each + min(xcd, more) + at;
-    const uint32_t panel = id / (kPanel * tiles_n), in = id - panel * kPanel * tiles_n;
-    const uint32_t rows = min(kPanel, tiles_m - panel * kPanel);
-    tn = in / rows;
-    tm = panel * kPanel + in - tn * rows;
-}
+struct Walk {
+    uint32_t first, count, at, step, tiles_m, tiles_n;
+    __device__ Walk(uint32_t m, uint32_t n) : tiles_m(m), tiles_n(n) {
+        const uint32_t total = m * n, each = total / 8, more = total % 8, xcd = blockIdx.x % 8;
+        first = xcd * each + min(xcd, more);
+        count = each + (xcd < more ? 1 : 0);
+        at = blockIdx.x / 8;
+        step = gridDim.x / 8;
+    }
+    __device__ __forceinline__ bool here() const { return at < count; }
+    __device__ __forceinline__ void tile(uint32_t& tm, uint32_t& tn) const {
+        const uint32_t id = first + at, panel = id / (kPanel * tiles_n), in = id - panel * kPanel * tiles_n;
+        const uint32_t rows = min(kPanel, tiles_m - panel * kPanel);
+        tn = in / rows;
+        tm = panel * kPanel + in - tn * rows;
+    }
+};
 
-// A BM x BN tile of c, waves of WM x 64, one block of 128 coordinates per step, two stages of LDS in turn: the copies of the next block are
-// in flight while the matrix cores work on this one.
+// BM x BN tiles of c, waves of WM x 64, a block of 128 coordinates per step, two stages of LDS in turn.
+//
+// Rows: fragment i of a wave's WM rows is rows i, i + FM, i + 2 FM ... of them (FM = WM / 16): the FM rows of a lane are neighbours, their
+// scale bytes one or two dwords, and the matrix cores pick the byte.  The same for the points, so a lane ends up with 16 consecutive
+// columns of each of its rows and writes them itself.
+// LDS: fragment by fragment, a row's 128 codes as 8 chunks of 16 bytes, chunk c of LDS row r at place c ^ ((r >> 1) & 7): 16 lanes that read the
+// same chunk of 16 rows touch all 64 banks once.  The copies to LDS write lane after lane, so the lanes permute what they fetch.
+// Rows beyond the operands and bytes beyond a row lie outside the buffers' range and read as 0.
+//
+// The blocks of all tiles of a workgroup form one stream: the copy runs two blocks ahead of the products, across the end of a tile, and the
+// stores of a tile drain under the next one.  A step's fragment is read two steps ahead.  Two steps before its end a block's stage has been read by
+// everybody and the next one has to be there: one barrier a block.  The loop's body has no branch (copies beyond the last tile fetch nothing).
 template <int TYPE, int BM, int BN, int WM>
 __global__ void __launch_bounds__((BM / WM) * (BN / 64) * 64, (BM + BN) * kBlock * 2 > 80 * 1024 ? (BM / WM) * (BN / 64) / 4 : (BM / WM) * (BN / 64) / 2)
 product_tile_kernel(ProductArgs a) {
-    constexpr int WN = 64, WAVES = (BM / WM) * (BN / WN), FM = WM / 32, FN = WN / 32;
+    constexpr int WN = 64, WAVES = (BM / WM) * (BN / WN), FM = WM / 16, FN = WN / 16;
     constexpr int STAGE = (BM + BN) * kBlock;
-    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
+    constexpr bool EXACT = TYPE == AE_TYPE_F32;
+    constexpr int STEPS = EXACT ? 2 * FM : FM;   // a step: FM-th part of the rows, the whole block or (f32) a half of it
     using T = typename Elem<TYPE>::T;
-    uint32_t tm, tn;
-    tile_of(a.tiles_m, a.tiles_n, tm, tn);
-    const uint64_t i0 = (uint64_t)tm * BM, j0 = (uint64_t)tn * BN;
-    const int mi = (int)min((uint64_t)BM, a.x.rows - i0), nj = (int)min((uint64_t)BN, a.p.rows - j0);
+    constexpr int STORES = FM * (int)sizeof(T);
+    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
+    Walk walk(a.tiles_m, a.tiles_n);
+    if (!walk.here()) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = (wave / (BN / WN)) * WM, wj = (wave % (BN / WN)) * WN;
-    // rows beyond the tile and bytes beyond a row are outside the buffers' range: they read as 0
     const uint32_t stride = (uint32_t)a.x.row_bytes;
-    __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x.codes + i0 * stride), (short)0, (int)((uint32_t)mi * stride), 0x00027000);
-    __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.codes + j0 * stride), (short)0, (int)((uint32_t)nj * stride), 0x00027000);
-    static_assert(WAVES % 2 == 0 && BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0, "a wave copies whole groups of 8 rows of one operand");
-    const uint32_t chunk = (lane & 7) ^ (((wave & 1) << 2) + (lane >> 4));   // (row >> 1) & 7 of row = 8 (q WAVES + wave) + (lane >> 3)
-    const uint32_t lane_off = (uint32_t)(wave * 8 + (lane >> 3)) * stride + chunk * 16;
-    auto fetch = [&](uint32_t kb, uint8_t* to) {
-        const bool in = kb * kBlock + chunk * 16 < stride;
+
+    // ---- the copies
+    static_assert(WAVES % 2 == 0 && BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0 && FM % 4 == 0 && FN == 4, "");
+    const uint32_t chunk = (lane & 7) ^ (((wave & 1) << 2) + (lane >> 4));   // (r >> 1) & 7 of LDS row r = 8 (q WAVES + wave) + (lane >> 3)
+    const uint32_t row16 = (wave & 1) * 8 + (lane >> 3);                     // r % 16
+    Walk ahead = walk;
+    uint32_t ahead_kb = 0, off_k, off_x, off_p;
+    __amdgpu_buffer_rsrc_t rx, rp;
+    auto aim = [&]() {   // the copies turn to the tile `ahead`; past the last one to nothing
+        uint32_t tm = 0, tn = 0;
+        ahead.tile(tm, tn);
+        const bool on = ahead.here();
+        const uint64_t i0 = on ? (uint64_t)tm * BM : 0, j0 = on ? (uint64_t)tn * BN : 0;
+        const uint32_t mi = on ? (uint32_t)min((uint64_t)BM, a.x.rows - i0) : 0, nj = on ? (uint32_t)min((uint64_t)BN, a.p.rows - j0) : 0;
+        rx = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x.codes + i0 * stride), (short)0, (int)(mi * stride), 0x00027000);
+        rp = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.codes + j0 * stride), (short)0, (int)(nj * stride), 0x00027000);
+        off_k = chunk * 16;
+        off_x = row16 * FM * stride + off_k;
+        off_p = row16 * FN * stride + off_k;
+    };
+    auto copy = [&](uint32_t stage) {   // the next block of the stream
+        const bool in = off_k < stride;
 #pragma unroll
         for (int q = 0; q < (BM + BN) / 8 / WAVES; q++) {
             const bool of_x = q < BM / 8 / WAVES;
-            const uint32_t off = lane_off + (uint32_t)((of_x ? q : q - BM / 8 / WAVES) * WAVES * 8) * stride + kb * kBlock;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(of_x ? rx : rp, (__attribute__((address_space(3))) void*)(to + (q * WAVES + wave) * 8 * kBlock), 16, (int)(in ? off : 0x7FFFFFFFu), 0, 0, 0);
+            const uint32_t r0 = ((of_x ? q : q - BM / 8 / WAVES) * WAVES + wave) * 8;
+            const uint32_t first = of_x ? r0 / WM * WM + r0 % WM / 16 : r0 / WN * WN + r0 % WN / 16;
+            const uint32_t off = (of_x ? off_x : off_p) + first * stride;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(of_x ? rx : rp, (__attribute__((address_space(3))) void*)(lds + stage * STAGE + (q * WAVES + wave) * 8 * kBlock), 16,
+                                                     (int)(in ? off : 0x7FFFFFFFu), 0, 0, 0);
+        }
+        off_k += kBlock;
+        off_x += kBlock;
+        off_p += kBlock;
+    };
+    auto advance = [&]() {
+        if (++ahead_kb == a.blocks) {
+            ahead_kb = 0;
+            ahead.at += ahead.step;
+            aim();
         }
     };
-    f32x16 acc[FM][FN];
+
+    // ---- the tile's scales: one block ahead
+    uint32_t tm, tn;
+    walk.tile(tm, tn);
+    const uint8_t* sx = a.x.scales + (uint64_t)tm * BM + wi;
+    const uint8_t* sp = a.p.scales + (uint64_t)tn * BN + wj;
+    const uint32_t at_x = (lane & 15) * FM, at_p = (lane & 15) * FN;
+    uint32_t nx[FM / 4], np[1], bx[FM / 4], bp[1];
+    auto scales = [&]() {
+        __builtin_memcpy(nx, sx + at_x, FM);
+        __builtin_memcpy(np, sp + at_p, FN);
+    };
+
+    // ---- fragments
+    f32x4 acc[FM][FN];
+    auto clear = [&]() {
 #pragma unroll
-    for (int i = 0; i < FM; i++)
+        for (int i = 0; i < FM; i++)
 #pragma unroll
-        for (int j = 0; j < FN; j++)
+            for (int j = 0; j < FN; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    i32x8 fx[4], fp[FN];        // of f32 only the first halves
+    bf16x8 wp[FN][2];           // f32: the points' values of half a block
+    const int r_x = wi + (lane & 15), r_p = BM + wj + (lane & 15), c0 = (lane >> 4) * 2;
+    uint32_t in_x = r_x * kBlock + ((c0 ^ ((r_x >> 1) & 7)) << 4), in_p = r_p * kBlock + ((c0 ^ ((r_p >> 1) & 7)) << 4);
+    auto chunk_at = [&](uint32_t at) { return *reinterpret_cast<const u32x4*>(lds + at); };
+    auto read_x = [&](int s) {
+        if constexpr (EXACT) fx[s & 3] = join(chunk_at((in_x ^ (s / FM * 16)) + s % FM * 16 * kBlock), u32x4{0, 0, 0, 0});
+        else fx[s & 3] = join(chunk_at(in_x + s * 16 * kBlock), chunk_at((in_x ^ 16) + s * 16 * kBlock));
+    };
+    auto read_p = [&](int j, int h) {
+        if constexpr (EXACT) fp[j] = join(chunk_at((in_p ^ (h * 16)) + j * 16 * kBlock), u32x4{0, 0, 0, 0});
+        else fp[j] = join(chunk_at(in_p + j * 16 * kBlock), chunk_at((in_p ^ 16) + j * 16 * kBlock));
+    };
+    auto block = [&](uint32_t stage, auto first) {
 #pragma unroll
-            for (int t = 0; t < 16; t++) acc[i][j][t] = 0.f;
-    // scale bytes: a dword holds four blocks of a row; the next four are on their way while four are used
-    const uint32_t* sx[FM];
-    const uint32_t* sp[FN];
-    uint32_t nx[FM], np[FN], bx[FM], bp[FN];
+        for (int q = 0; q < FM / 4; q++) bx[q] = nx[q];
+        bp[0] = np[0];
+        scales();
 #pragma unroll
-    for (int i = 0; i < FM; i++) {
-        sx[i] = reinterpret_cast<const uint32_t*>(a.x.scales + (i0 + min(wi + i * 32 + (lane & 31), mi - 1)) * a.x.scale_stride);
-        nx[i] = sx[i][0];
-    }
-#pragma unroll
-    for (int j = 0; j < FN; j++) {
-        sp[j] = reinterpret_cast<const uint32_t*>(a.p.scales + (j0 + min(wj + j * 32 + (lane & 31), nj - 1)) * a.p.scale_stride);
-        np[j] = sp[j][0];
-    }
-    fetch(0, lds);
-    for (uint32_t kb = 0; kb < a.blocks; kb++) {
-        __syncthreads();   // this stage has arrived, everybody has left the other one
-        if ((kb & 3) == 0) {
-            const uint32_t next = min(kb / 4 + 1, (a.blocks - 1) / 4);
-#pragma unroll
-            for (int i = 0; i < FM; i++) { bx[i] = nx[i]; nx[i] = sx[i][next]; }
-#pragma unroll
-            for (int j = 0; j < FN; j++) { bp[j] = np[j]; np[j] = sp[j][next]; }
-        } else {
-#pragma unroll
-            for (int i = 0; i < FM; i++) bx[i] >>= 8;
-#pragma unroll
-            for (int j = 0; j < FN; j++) bp[j] >>= 8;
-        }
-        const uint8_t* t = lds + (kb & 1) * STAGE;
-        if (kb + 1 < a.blocks) fetch(kb + 1, lds + ((kb + 1) & 1) * STAGE);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            u32x4 fx[FM][2], fp[FN][2];
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int c = h * 4 + (lane >> 5) * 2 + e;
-#pragma unroll
-                for (int j = 0; j < FN; j++) fp[j][e] = *reinterpret_cast<const u32x4*>(t + swizzled(BM + wj + j * 32 + (lane & 31), c));
-#pragma unroll
-                for (int i = 0; i < FM; i++) fx[i][e] = *reinterpret_cast<const u32x4*>(t + swizzled(wi + i * 32 + (lane & 31), c));
+        for (int s = 0; s < STEPS; s++) {
+            if (s == STEPS - 2) {
+                // this wave's copies are in LDS; at a tile's first block the stores of the last one, issued after them, may go on
+                if constexpr (decltype(first)::value) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STORES) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): this wave's reads of the stage are done
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                copy(stage);
+                const uint32_t other = stage ? 0u - STAGE : STAGE;
+                in_x += other;
+                in_p += other;
             }
-            if constexpr (TYPE == AE_TYPE_F32) {
+            read_x((s + 2) % STEPS);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (EXACT) {
+                const int h = s / FM, i = s % FM;
+                if (i == 0) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {   // 8 codes of each operand
-                    bf16x8 wx[FM], wp[FN];
+                    for (int j = 0; j < FN; j++) {
 #pragma unroll
-                    for (int j = 0; j < FN; j++) wp[j] = widen8(fp[j][e >> 1][(e & 1) * 2], fp[j][e >> 1][(e & 1) * 2 + 1], bp[j] & 255u);
+                        for (int e = 0; e < 2; e++) wp[j][e] = widen8((uint32_t)fp[j][2 * e], (uint32_t)fp[j][2 * e + 1], byte_of(bp, j));
+                        if (h == 0) read_p(j, 1);
+                    }
+                }
 #pragma unroll
-                    for (int i = 0; i < FM; i++) wx[i] = widen8(fx[i][e >> 1][(e & 1) * 2], fx[i][e >> 1][(e & 1) * 2 + 1], bx[i] & 255u);
+                for (int e = 0; e < 2; e++) {
+                    const bf16x8 wx = widen8((uint32_t)fx[s & 3][2 * e], (uint32_t)fx[s & 3][2 * e + 1], byte_of(bx, i));
 #pragma unroll
-                    for (int i = 0; i < FM; i++)
+                    for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp[j][e], wx, acc[i][j], 0, 0, 0);
+                }
+                if (s == STEPS - 1) {
 #pragma unroll
-                        for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wp[j], wx[i], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < FN; j++) read_p(j, 0);
                 }
             } else {
-#pragma unroll
-                for (int i = 0; i < FM; i++)
-#pragma unroll
-                    for (int j = 0; j < FN; j++)
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(join(fp[j][0], fp[j][1]), join(fx[i][0], fx[i][1]), acc[i][j], 0, 0, 0, (int)bp[j], 0, (int)bx[i]);
+#define AE_STEP(J, I)                                                                                                                             \
+    acc[s][J] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp[J], fx[s & 3], acc[s][J], 0, 0, J, (int)bp[0], I, (int)bx[s >> 2]);           \
+    if (s == STEPS - 1) read_p(J, 0);
+#define AE_STEPS(I) AE_STEP(0, I) AE_STEP(1, I) AE_STEP(2, I) AE_STEP(3, I)
+                if ((s & 3) == 0) { AE_STEPS(0) }
+                else if ((s & 3) == 1) { AE_STEPS(1) }
+                else if ((s & 3) == 2) { AE_STEPS(2) }
+                else { AE_STEPS(3) }
+#undef AE_STEPS
+#undef AE_STEP
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-    }
-    // The points are the matrix cores' rows: a lane holds runs of 4 consecutive j of one row i.  A wave turns its part in a share of the
-    // stages and writes rows of 64 j, 16 bytes a lane.
+        // (the sums are taken note of here, or the compiler moves the products past what follows)
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) asm volatile("" : "+v"(acc[i][j]));
+    };
+
+    aim();
+    copy(0);
+    advance();
+    copy(1);
+    advance();
+    scales();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    constexpr int ROW = WN * sizeof(T), CH = ROW / 16;                      // bytes and 16-byte chunks of a row
-    constexpr int FIT = 2 * STAGE / WAVES / (32 * ROW);                      // fragments of 32 rows that a wave has room for
-    constexpr int STEP = FIT >= FM ? FM : FIT >= FM / 2 ? FM / 2 : 1;
-    static_assert(WAVES * STEP * 32 * ROW <= 2 * STAGE, "the turned tiles fit in the stages");
-    uint8_t* mine = lds + wave * (STEP * 32 * ROW);
-    T* c = static_cast<T*>(a.c);
-    auto place = [&](int r, int ch) { return r * ROW + ((ch ^ (ROW == 128 ? (r >> 1) & 7 : r & 15)) << 4); };
 #pragma unroll
-    for (int i = 0; i < FM; i += STEP) {
-#pragma unroll
-        for (int f = 0; f < STEP; f++)
-#pragma unroll
-            for (int j = 0; j < FN; j++)
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    using V = __attribute__((ext_vector_type(4))) T;
-                    V v;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = (T)acc[i + f][j][q * 4 + e];
-                    const int byte = (j * 32 + q * 8 + (lane >> 5) * 4) * (int)sizeof(T);
-                    *reinterpret_cast<V*>(mine + place(f * 32 + (lane & 31), byte >> 4) + (byte & 15)) = v;
-                }
-        // (within a wave LDS operations are in order)
-#pragma unroll
-        for (int q = 0; q < STEP * 32 * CH / 64; q++) {
-            const int at = q * 64 + lane, r = at / CH, ch = at % CH;
-            const int row = wi + i * 32 + r, col = wj + ch * (16 / (int)sizeof(T));
-            const u32x4 v = *reinterpret_cast<const u32x4*>(mine + place(r, ch));
-            if (row >= mi || col >= nj) continue;
-            T* to = c + (i0 + row) * a.ldc + j0 + col;
-            if (a.vec && col + 16 / (int)sizeof(T) <= nj) *reinterpret_cast<u32x4*>(to) = v;
-            else {
-                const T* one = reinterpret_cast<const T*>(&v);
-#pragma unroll
-                for (int e = 0; e < 16 / (int)sizeof(T); e++)
-                    if (col + e < nj) to[e] = one[e];
+    for (int j = 0; j < FN; j++) read_p(j, 0);
+    read_x(0);
+    read_x(1);
+    uint32_t stage = 0;
+    for (;;) {
+        const uint64_t i0 = (uint64_t)tm * BM, j0 = (uint64_t)tn * BN;
+        clear();
+        walk.at += walk.step;
+        const bool more = walk.here();
+        if (more) walk.tile(tm, tn);
+        auto scales_turn = [&](uint32_t kb) {   // the scales' pointers go to the block after kb
+            sx += a.x.scale_stride;
+            sp += a.p.scale_stride;
+            if (kb + 1 == a.blocks) {   // (the last tile's last block takes scales nobody uses)
+                sx = a.x.scales + (uint64_t)tm * BM + wi;
+                sp = a.p.scales + (uint64_t)tn * BN + wj;
             }
+        };
+        scales_turn(0);
+        block(stage, std::true_type{});
+        stage ^= 1;
+        advance();
+        for (uint32_t kb = 1; kb < a.blocks; kb++) {
+            scales_turn(kb);
+            block(stage, std::false_type{});
+            stage ^= 1;
+            advance();
         }
+        // c: lane (i, g) holds columns 16 g ... 16 g + 15 of rows i FM ... i FM + FM - 1 of the wave's part, column 4 q + j in acc[.][j][q]
+        T* c = static_cast<T*>(a.c) + i0 * a.ldc + j0;
+        const int mi = (int)min((uint64_t)BM, a.x.rows - i0), nj = (int)min((uint64_t)BN, a.p.rows - j0);
+        constexpr int W = 16 / sizeof(T);
+        const int row = wi + (lane & 15) * FM, col = wj + (lane >> 4) * 16;
+        if (a.vec && (nj == BN || nj % W == 0)) {
+            __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)c, (short)0, (int)(((uint32_t)(mi - 1) * (uint32_t)a.ldc + (uint32_t)nj) * (uint32_t)sizeof(T)), 0x00027000);
+            // the four lanes of a row change 16-byte pieces among them, so that a store writes 64 consecutive bytes of 16 rows
+            const int piece = wj + (lane >> 4) * W;
+#pragma unroll
+            for (int i = 0; i < FM; i++) {
+                u32x4 v[16 / W];
+#pragma unroll
+                for (int q = 0; q < 16 / W; q++) {
+                    using V = __attribute__((ext_vector_type(W))) T;
+                    V one;
+#pragma unroll
+                    for (int e = 0; e < W; e++) one[e] = (T)acc[i][(q * W + e) & 3][(q * W + e) >> 2];
+                    v[q] = __builtin_bit_cast(u32x4, one);
+                }
+                if constexpr (W == 4) { swap32(v[0], v[2]); swap32(v[1], v[3]); swap16(v[0], v[1]); swap16(v[2], v[3]); }
+                else { swap16(v[0], v[1]); swap32(v[0], v[1]); }
+#pragma unroll
+                for (int q = 0; q < 16 / W; q++) {
+                    const int at = piece + q * 4 * W;
+                    const uint32_t off = ((uint32_t)(row + i) * (uint32_t)a.ldc + (uint32_t)at) * (uint32_t)sizeof(T);
+                    __builtin_amdgcn_raw_buffer_store_b128(v[q], rc, (int)(at < nj ? off : 0x7FFFFFFFu), 0, 0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < FM; i++)
+#pragma unroll
+                for (int q = 0; q < 16; q++)
+                    if (row + i < mi && col + q < nj) c[(uint64_t)(row + i) * a.ldc + col + q] = (T)acc[i][q & 3][q >> 2];
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (an unknown number of stores: none may be in flight where STORES of them are allowed for)
+        }
+        if (!more) break;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the copies of nothing have ended before the LDS is given back
 }
 
 template <int BM, int BN, int WM>
 void launch_tiles(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t ctype, uint64_t ldc, hipStream_t s) {
-    const uint64_t tiles_m = (x.rows + BM - 1) / BM, tiles_n = (p.rows + BN - 1) / BN;
-    if (tiles_m * tiles_n > 0x3FFFFFull) fail(AE_ERR_INVALID_ARG, "ae_points8_product: %llu x %llu are more products than one call takes", (unsigned long long)x.rows, (unsigned long long)p.rows);
-    const ProductArgs a{x, p, points8_blocks(dim), d_c, ldc, (uint32_t)tiles_m, (uint32_t)tiles_n, vector_rows(d_c, ctype, ldc) ? 1u : 0u};
-    constexpr unsigned threads = (BM / WM) * (BN / 64) * 64, bytes = 2 * (BM + BN) * kBlock;
+    const uint64_t tiles_m = (x.rows + BM - 1) / BM, tiles_n = (p.rows + BN - 1) / BN, tiles = tiles_m * tiles_n;
+    if (tiles > 0x3FFFFFFFull) fail(AE_ERR_INVALID_ARG, "ae_points8_product: %llu x %llu are more products than one call takes", (unsigned long long)x.rows, (unsigned long long)p.rows);
+    constexpr unsigned threads = (BM / WM) * (BN / 64) * 64, bytes = 2 * (BM + BN) * kBlock, resident = 256 * (bytes > 80 * 1024 ? 1 : 2);
+    const bool vec = vector_rows(d_c, ctype, ldc) && ldc * type_size(ctype) < 0x7FFF0000ull / BM;
+    const ProductArgs a{x, p, points8_blocks(dim), d_c, ldc, (uint32_t)tiles_m, (uint32_t)tiles_n, vec ? 1u : 0u};
+    const unsigned grid = tiles < resident ? (unsigned)((tiles + 7) / 8 * 8) : resident;
     by_type(ctype, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
-        hipLaunchKernelGGL((product_tile_kernel<TYPE, BM, BN, WM>), dim3((unsigned)(tiles_m * tiles_n)), dim3(threads), bytes, s, a);
+        hipLaunchKernelGGL((product_tile_kernel<TYPE, BM, BN, WM>), dim3(grid), dim3(threads), bytes, s, a);
     });
     check_launch("points8_product");
 }
 
+// 256 x 256 tiles read every operand least often but leave one workgroup on a CU: taken where they fill the chip and their edges waste
+// little (4096 x 4096 x 1024 to bf16: 21.6 against 23.9 us with 128 x 128, 8192^3: 418 against 585; 1024 x 10 000 x 784, 160 tiles: 20.5
+// against 19.4; 300 x 60 000 x 784, two rows of tiles for 300: 35.3 against 30.9).
 void product(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t ctype, uint64_t ldc, hipStream_t s) {
-    const char* v = debug_knob("AE_P8");
-    const int w = v ? atoi(v) : 1;
-    if (w == 2) launch_tiles<256, 256, 128>(x, p, dim, d_c, ctype, ldc, s);
-    else if (w == 3) launch_tiles<64, 256, 64>(x, p, dim, d_c, ctype, ldc, s);
-    else if (w == 4) launch_tiles<128, 256, 64>(x, p, dim, d_c, ctype, ldc, s);
+    const uint64_t tm = (x.rows + 255) / 256, tn = (p.rows + 255) / 256;
+    if (tm * tn >= 256 && tm * 256 * 4 <= x.rows * 5 && tn * 256 * 4 <= p.rows * 5) launch_tiles<256, 256, 128>(x, p, dim, d_c, ctype, ldc, s);
     else launch_tiles<128, 128, 64>(x, p, dim, d_c, ctype, ldc, s);
 }
 
-uint64_t product_work(uint64_t m, uint64_t dim) { return m * (points8_row_bytes(dim) + points8_scale_stride(dim)); }
+uint64_t product_work(uint64_t m, uint64_t dim) { return m * points8_row_bytes(dim) + points8_blocks(dim) * points8_scale_stride(m) + kScaleSlack; }
 
 }  // namespace
 
@@ -241,8 +366,8 @@ int32_t ae_points8_product(const ae_points8* p, uint64_t first, uint64_t n, cons
         check_aligned(d_work, 16, "ae_points8_product: work");
         uint8_t* codes = static_cast<uint8_t*>(d_work);
         uint8_t* scales = codes + m * p->row_bytes;
-        points8_quantise(d_x, xtype, m, ldx, p->dim, codes, scales, (hipStream_t)stream);
-        product(Rows8{codes, scales, p->row_bytes, p->scale_stride, m}, points8_rows(p, first, n), p->dim, d_c, ctype, ldc, (hipStream_t)stream);
+        points8_quantise(d_x, xtype, m, ldx, p->dim, codes, scales, points8_scale_stride(m), (hipStream_t)stream);
+        product(Rows8{codes, scales, p->row_bytes, points8_scale_stride(m), m}, points8_rows(p, first, n), p->dim, d_c, ctype, ldc, (hipStream_t)stream);
     });
 }
 

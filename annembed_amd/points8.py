@@ -90,9 +90,9 @@ class _Store:
 
 
 class _View:
-    def __init__(self, store, ptr, shape, stride):
+    def __init__(self, store, ptr, shape, strides):
         self.store = store
-        self.__cuda_array_interface__ = {"shape": shape, "strides": (stride, 1), "typestr": "|u1", "data": (ptr, False), "version": 2}
+        self.__cuda_array_interface__ = {"shape": shape, "strides": strides, "typestr": "|u1", "data": (ptr, False), "version": 2}
 
 
 class Points8:
@@ -115,9 +115,9 @@ class Points8:
             check(L.load().ae_points8_info(h, None, None, C.byref(row_bytes), C.byref(stride)))
             check(L.load().ae_points8_device(h, C.byref(codes), C.byref(scales)))
             blocks = -(-self.dim // 128)
-            c = torch.as_tensor(_View(self._store, codes.value, (self.capacity, self.dim), row_bytes.value), device=self.device)
+            c = torch.as_tensor(_View(self._store, codes.value, (self.capacity, self.dim), (row_bytes.value, 1)), device=self.device)
             self._codes = c.view(torch.float8_e4m3fn)
-            self._scales = torch.as_tensor(_View(self._store, scales.value, (self.capacity, blocks), stride.value), device=self.device)
+            self._scales = torch.as_tensor(_View(self._store, scales.value, (self.capacity, blocks), (1, stride.value)), device=self.device)
 
     @property
     def handle(self):

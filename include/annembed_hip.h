@@ -610,9 +610,9 @@ typedef struct ae_points8 ae_points8;
 /* room for `capacity` rows (< 2^32 - 1) of `dim` coordinates (1 ... 2^20) on the current device, all of them zero.  Synchronous. */
 int32_t ae_points8_create(uint64_t capacity, uint64_t dim, ae_points8 **out);
 int32_t ae_points8_destroy(ae_points8 *p);
-/* row_bytes: bytes from row to row of the codes (dim rounded up to 16); scale_stride: from row to row of the scale bytes */
+/* row_bytes: bytes from row to row of the codes (dim rounded up to 16); scale_stride: bytes from block to block of the scales */
 int32_t ae_points8_info(const ae_points8 *p, uint64_t *capacity, uint64_t *dim, uint64_t *row_bytes, uint64_t *scale_stride);
-/* the device memory itself: codes[capacity][row_bytes], scales[capacity][scale_stride] */
+/* the device memory itself: codes[capacity][row_bytes], scales[blocks of a row][scale_stride], a byte for each row */
 int32_t ae_points8_device(const ae_points8 *p, void **d_codes, void **d_scales);
 /* Row i of x (n rows of dim values) goes to row d_slots[i] of the store, or to row first + i where d_slots is NULL.  A slot outside the
    store (0xFFFFFFFF marks padding) is skipped; where a slot comes several times the LAST of its rows is held.  Other rows stay as they are.
