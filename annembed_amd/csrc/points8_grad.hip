@@ -5,10 +5,10 @@
 // compute the product of the values themselves with f32 sums: nothing is rounded before the result.
 //
 // A workgroup owns 64 FR rows x 128 coordinates (one block: one scale byte per point) and walks a slice of the points 64 at a time; a wave owns
-// 16 FR of the rows and all coordinates.  dc never touches LDS: a lane's 8 consecutive points of a row are the matrix cores' operand as they
-// lie in memory.  The codes are turned on the way to LDS: a thread takes 4 coordinates of 8 points, widens them and writes 8 points of one
-// coordinate as 16 bytes.  Both are fetched two steps ahead into the registers that the step frees.  Few rows leave few tiles: the points are
-// split into slices whose sums are joined in order.
+// 16 FR of the rows and all coordinates.  dc goes to LDS as it is, three steps deep.  (Straight to the lanes that multiply it, 16 bytes of 16
+// rows each, every lane would be an access of its own to the cache: 57 us where this takes 4x fewer.)  The codes are turned on the way to LDS:
+// a thread takes 4 coordinates of 8 points, widens them under the products of the step before and writes 8 points of one coordinate as 16
+// bytes.  One barrier a step.  Few rows leave few tiles: the points are split into slices whose sums are joined in order.
 #include "points8.h"
 
 #include <algorithm>
@@ -18,12 +18,17 @@ using namespace ae;
 namespace {
 
 constexpr int kStep = 64;    // points per step: 128 bytes of bf16
-constexpr uint32_t kOutside = 0x80000000u;   // or-ed into an offset: outside every buffer's range (they span less than 2 GiB)
+constexpr uint32_t kOutside = 0x40000000u;   // an offset outside every buffer's range (dc's rows of a tile, a slice's codes: less than 1 GiB)
 
 template <int TYPE> constexpr int terms_of() { return TYPE == AE_TYPE_F32 ? 3 : TYPE == AE_TYPE_F16 ? 2 : 1; }
 
-// a coordinate's 64 points as 8 chunks of 16 bytes; written four coordinates apart, read coordinate after coordinate, both without bank conflicts
+// The 64 points of a step are 8 chunks of 8.  Lane group g takes chunk part(h, g) of half h, of dc and of the coordinates alike: with these and
+// the places below the 16 lanes that LDS serves at a time (0-3, 12-15 and 20-27 of a half wave, then the others) touch all 64 banks once.
+__device__ __forceinline__ int part(int h, int g) { return ((h ? 0x4352 : 0x6170) >> (g * 4)) & 7; }
+// a coordinate's chunks of 16 bytes: written four coordinates apart, read coordinate after coordinate
 __device__ __forceinline__ int at_coords(int k, int chunk) { return k * 128 + ((chunk ^ ((k >> 2) & 7) ^ ((k & 2) << 1)) << 4); }
+// a row of dc: 8 (f32: 16) pieces of 16 bytes
+template <int PIECES> __device__ __forceinline__ int turn(int r) { return PIECES == 8 ? (r >> 1) & 7 : r & 15; }
 
 // eight values as the sum of TERMS bf16 numbers, the first ones cut off (never past the largest bf16): exact apart from what lies below bf16's range
 template <int TYPE>
@@ -57,11 +62,13 @@ struct GradArgs {
     uint32_t tiles_k, tiles, slices;
 };
 
-template <int TYPE, int FR, bool VEC>   // VEC: rows of dc lie on 16 bytes, 64 FR of them and a slice's codes span less than 2 GiB
-__global__ void __launch_bounds__(256, FR <= 2 ? 2 : 1) grad_tile_kernel(GradArgs a) {
+template <int TYPE, int FR> constexpr int grad_lds() { return 3 * 64 * FR * kStep * (TYPE == AE_TYPE_F32 ? 4 : 2) + 2 * kBlock * 128; }
+
+template <int TYPE, int FR, bool VEC>   // VEC: rows of dc lie on 16 bytes, 64 FR of them span less than 1 GiB
+__global__ void __launch_bounds__(256, (grad_lds<TYPE, FR>() <= 80 * 1024 ? 2 : 1)) grad_tile_kernel(GradArgs a) {
     using T = typename Elem<TYPE>::T;
-    constexpr int TERMS = terms_of<TYPE>(), PIECES = (int)sizeof(T) / 2;   // 16-byte pieces of 8 values
-    __shared__ __attribute__((aligned(128))) uint8_t lds[2][kBlock * 128];
+    constexpr int TERMS = terms_of<TYPE>(), ROW = kStep * (int)sizeof(T), PIECES = ROW / 16, STAGE = 64 * FR * ROW, COPIES = STAGE / 4096;
+    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];   // three stages of dc, two of coordinates
     // Workgroups go to the 8 XCDs in turn, each with an L2 of its own: an XCD owns a run of slices, all tiles of a slice one after the other, so
     // that dc and the points are fetched from memory once and shared there.
     const uint32_t total = a.tiles * a.slices, each = total / 8, more = total % 8, xcd = blockIdx.x % 8, at = blockIdx.x / 8;
@@ -69,59 +76,57 @@ __global__ void __launch_bounds__(256, FR <= 2 ? 2 : 1) grad_tile_kernel(GradArg
     const uint32_t id = xcd * each + min(xcd, more) + at, slice = id / a.tiles, tile = id - slice * a.tiles, ti = tile / a.tiles_k, tk = tile - ti * a.tiles_k;
     const uint64_t i0 = (uint64_t)ti * (64 * FR), k0 = (uint64_t)tk * kBlock;
     const uint64_t jb = slice * a.per_slice, je = min(a.n, jb + a.per_slice);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     const int kg = tid & 31, jg = tid >> 5;   // this thread's 4 coordinates and 8 points
     const uint32_t mi = (uint32_t)min((uint64_t)(64 * FR), a.m - i0), points = (uint32_t)(je - jb), steps = (points + kStep - 1) / kStep;
     const int r0 = wave * 16 * FR + (lane & 15);   // this lane's first row of the tile; the others 16 apart
     const T* dc = static_cast<const T*>(a.dc) + i0 * a.lddc + jb;
-    // Rows beyond m and pieces behind the last point lie outside the buffer's range, or are put there.  The piece with the last point is fetched
-    // whole -- it lies on 16 bytes, so in one page -- and cut.
+    // Rows beyond m lie outside the buffer's range, which ends with the piece of the last row's last point: it is fetched whole (it lies on
+    // 16 bytes, so in one page).  A lane's offsets never change, the step goes into the scalar one, which stays inside the range (steps past the
+    // last one fetch the last again, for nobody).  What is fetched behind the last point is cut in the last step.
     const uint32_t row_bytes = (uint32_t)a.lddc * (uint32_t)sizeof(T);
     __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)dc, (short)0, VEC ? (int)((mi - 1) * row_bytes + (points * (uint32_t)sizeof(T) + 15) / 16 * 16) : 0, 0x00027000);
     __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.codes + jb * a.p.row_bytes), (short)0, (int)(points * (uint32_t)a.p.row_bytes), 0x00027000);
-    const uint32_t code_at = (uint32_t)k0 + kg * 4;
+    const uint32_t k_at = (uint32_t)k0 + kg * 4, code_at = (uint32_t)(jg * 8) * (uint32_t)a.p.row_bytes + (k_at < a.p.row_bytes ? k_at : kOutside);
     const uint8_t* sc = a.p.scales + tk * a.p.scale_stride + jb + jg * 8;
-    const uint32_t k_out = code_at < a.p.row_bytes ? 0u : kOutside;
-    struct Fragment { u32x4 piece[2][PIECES]; };   // 8 points of a row in each half of the step
-    struct Codes { uint32_t code[8]; uint2 bytes; };
-    Fragment fa[2][FR];
-    Codes fc[2];
-    auto load_row = [&](uint32_t step, int i, Fragment& f) {
-        const uint32_t r = r0 + i * 16;
+    const int copy_row = wave * (64 / PIECES) + lane / PIECES, copy_piece = (lane % PIECES) ^ turn<PIECES>(copy_row);   // (copies are a multiple of 16 rows apart)
+    auto copy = [&](uint32_t step, uint32_t stage) {
+        step = min(step, steps - 1);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const uint32_t j = step * kStep + h * 32 + (lane >> 4) * 8;
-            if constexpr (VEC) {
+        for (int q = 0; q < COPIES; q++) {
+            const uint32_t r = q * (256 / PIECES) + copy_row;
+            uint8_t* to = lds + stage * STAGE + (q * 4 + wave) * 1024;
+            if constexpr (VEC)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rd, (__attribute__((address_space(3))) void*)to, 16, (int)(r * row_bytes + copy_piece * 16), (int)(step * ROW), 0, 0);
+            else {
+                constexpr int W = 16 / sizeof(T);
+                T v[W];
+                const uint32_t j = step * kStep + copy_piece * W;
 #pragma unroll
-                for (int q = 0; q < PIECES; q++) {
-                    const uint32_t jq = j + q * (8 / PIECES);
-                    f.piece[h][q] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rd, (int)((r * row_bytes + jq * (uint32_t)sizeof(T)) | (jq < points ? 0u : kOutside)), 0, 0));
-                }
-            } else {
-                T v[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = r < mi && j + e < points ? dc[r * a.lddc + j + e] : (T)0.f;
-                __builtin_memcpy(f.piece[h], v, sizeof(v));
+                for (int e = 0; e < W; e++) v[e] = r < mi && j + e < points ? dc[r * a.lddc + j + e] : (T)0.f;
+                __builtin_memcpy(to + lane * 16, v, 16);
             }
         }
     };
+    struct Codes { uint32_t code[8]; uint2 bytes; };
+    Codes fc[2];
     auto load_codes = [&](uint32_t step, Codes& c) {
-        const uint32_t j = step * kStep + jg * 8;
+        step = min(step, steps - 1);
 #pragma unroll
-        for (int e = 0; e < 8; e++) c.code[e] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rc, (int)(((j + e) * (uint32_t)a.p.row_bytes + code_at) | k_out), 0, 0);
-        __builtin_memcpy(&c.bytes, sc + min(step, steps) * kStep, 8);   // (bytes of points that do not exist multiply zeros; kScaleSlack)
+        for (int e = 0; e < 8; e++) c.code[e] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rc, (int)(code_at + e * (uint32_t)a.p.row_bytes), (int)(step * kStep * (uint32_t)a.p.row_bytes), 0);
+        __builtin_memcpy(&c.bytes, sc + step * kStep, 8);   // (bytes of points that do not exist multiply zeros; kScaleSlack)
     };
-    auto widen = [&](const Codes& c, uint8_t* to) {
+    uint8_t* const coords = lds + 3 * STAGE;
+    // part 0 ... 7: a point's 4 coordinates as bf16; part 8 ... 11: the 8 points of a coordinate to LDS
+    uint32_t wide[8][2];   // [point][coordinates 0, 1 | 2, 3]
+    auto widen = [&](int part, const Codes& c, uint8_t* to) {
         using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
-        uint32_t wide[8][2];   // [point][coordinates 0, 1 | 2, 3]
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float scale = __uint_as_float(((e < 4 ? c.bytes.x >> (e * 8) : c.bytes.y >> (e * 8 - 32)) & 255u) << 23);
-            wide[e][0] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.code[e], scale, false));
-            wide[e][1] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.code[e], scale, true));
-        }
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
+        if (part < 8) {
+            const float scale = __uint_as_float(((part < 4 ? c.bytes.x >> (part * 8) : c.bytes.y >> (part * 8 - 32)) & 255u) << 23);
+            wide[part][0] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.code[part], scale, false));
+            wide[part][1] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.code[part], scale, true));
+        } else {
+            const int t = part - 8;
             u32x4 w;
 #pragma unroll
             for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(wide[2 * e + 1][t >> 1], wide[2 * e][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
@@ -133,47 +138,77 @@ __global__ void __launch_bounds__(256, FR <= 2 ? 2 : 1) grad_tile_kernel(GradArg
     for (int i = 0; i < FR; i++)
 #pragma unroll
         for (int q = 0; q < 8; q++) acc[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto step = [&](uint32_t t, auto which, auto last) {
-        constexpr int S = decltype(which)::value;
-        widen(fc[S], lds[S]);
-        load_codes(t + 2, fc[S]);
-        __syncthreads();   // (the other buffer's readers have passed it too: one barrier a step)
-        bf16x8 terms[FR][2][TERMS];
+    bf16x8 fp[4];                   // 16 coordinates x 32 points, read two ahead
+    u32x4 raw[2][FR][PIECES / 8];   // 8 points of this lane's rows, of both halves
+    bf16x8 terms[FR][TERMS];        // of the half at work
+    auto read_coords = [&](const uint8_t* from, int x) { fp[x & 3] = *reinterpret_cast<const bf16x8*>(from + at_coords((x & 7) * 16 + (lane & 15), part(x >> 3, g))); };
+    auto read_rows = [&](const uint8_t* from, int h) {
 #pragma unroll
         for (int i = 0; i < FR; i++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                T v[8];
-                __builtin_memcpy(v, fa[S][i].piece[h], sizeof(v));
-                if constexpr (VEC && decltype(last)::value) {   // cut what lies behind the last point
-#pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = t * kStep + h * 32 + (lane >> 4) * 8 + e < points ? v[e] : (T)0.f;
-                }
-                split8<TYPE>(v, terms[i][h]);
+            for (int q = 0; q < PIECES / 8; q++) {
+                const int r = r0 + i * 16;
+                raw[h][i][q] = *reinterpret_cast<const u32x4*>(from + r * ROW + (((part(h, g) * (PIECES / 8) + q) ^ turn<PIECES>(r)) << 4));
             }
-        bf16x8 fp[4];   // 16 coordinates x 32 points, read two ahead
-        auto read = [&](int x) { fp[x & 3] = *reinterpret_cast<const bf16x8*>(lds[S] + at_coords((x & 7) * 16 + (lane & 15), (x >> 3) * 4 + (lane >> 4))); };
-        read(0);
-        read(1);
+    };
+    uint32_t stage = 0;   // of this step's dc
+    // A step is 16 parts: 16 coordinates over a half of the points.  Everything is read two parts ahead.  Two parts before its end a step's dc and
+    // coordinates have been read by everybody and the next one's have to be there.
+    auto step = [&](uint32_t t, auto which, auto last) {
+        constexpr int S = decltype(which)::value;
+        constexpr bool LAST = decltype(last)::value;
+        const uint32_t next = stage == 2 ? 0 : stage + 1;
+        if constexpr (!LAST) copy(t + 2, next == 2 ? 0 : next + 1);
 #pragma unroll
         for (int x = 0; x < 16; x++) {
-            if (x + 2 < 16) read(x + 2);
+            if (!LAST && x == 14) {
+                // all has arrived but what this step issued (COPIES copies, 9 loads of codes)
+                if constexpr (VEC) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COPIES + 9) : "memory");
+                __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            }
+            if (x < 14) read_coords(coords + S * (kBlock * 128), x + 2);
+            else if (!LAST) read_coords(coords + (S ^ 1) * (kBlock * 128), x - 14);
+            if (x == 4) read_rows(lds + stage * STAGE, 1);
+            if (!LAST && x == 14) read_rows(lds + next * STAGE, 0);
             __builtin_amdgcn_sched_barrier(0);
+            if ((x & 7) == 0) {
+#pragma unroll
+                for (int i = 0; i < FR; i++) {
+                    T v[8];
+                    __builtin_memcpy(v, raw[x >> 3][i], sizeof(v));
+                    if constexpr (VEC && LAST) {   // cut what lies behind the last point
+#pragma unroll
+                        for (int e = 0; e < 8; e++) v[e] = t * kStep + part(x >> 3, g) * 8 + e < points ? v[e] : (T)0.f;
+                    }
+                    split8<TYPE>(v, terms[i]);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < FR; i++)
 #pragma unroll
-                for (int u = TERMS - 1; u >= 0; u--) acc[i][x & 7] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[x & 3], terms[i][x >> 3][u], acc[i][x & 7], 0, 0, 0);
+                for (int u = TERMS - 1; u >= 0; u--) acc[i][x & 7] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[x & 3], terms[i][u], acc[i][x & 7], 0, 0, 0);
+            // under the products: the next step's coordinates
+            if (!LAST && x < 12) widen(x, fc[S ^ 1], coords + (S ^ 1) * (kBlock * 128));
+            if (!LAST && x == 8) load_codes(t + 3, fc[S ^ 1]);
             __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int i = 0; i < FR; i++) load_row(t + 2, i, fa[S][i]);
+        stage = next;
     };
+    load_codes(0, fc[0]);
+    load_codes(1, fc[1]);
+    asm volatile("" ::: "memory");
+    copy(0, 0);
+    copy(1, 1);
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
-        load_codes(s, fc[s]);
-#pragma unroll
-        for (int i = 0; i < FR; i++) load_row(s, i, fa[s][i]);
-    }
+    for (int x = 0; x < 12; x++) widen(x, fc[0], coords);
+    load_codes(2, fc[0]);
+    if constexpr (VEC) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    read_rows(lds, 0);
+    read_coords(coords, 0);
+    read_coords(coords, 1);
     constexpr std::integral_constant<int, 0> even;
     constexpr std::integral_constant<int, 1> odd;
     uint32_t t = 0;
@@ -185,6 +220,7 @@ __global__ void __launch_bounds__(256, FR <= 2 ? 2 : 1) grad_tile_kernel(GradArg
         step(t, even, std::false_type{});
         step(t + 1, odd, std::true_type{});
     } else step(t, even, std::true_type{});
+    if constexpr (VEC) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the copies for nobody have ended before the LDS is given back
     // coordinates are the matrix cores' rows: a lane holds runs of 4 consecutive k of its rows
     float* part = a.part + slice * (a.m * a.ldp);
 #pragma unroll
@@ -193,7 +229,7 @@ __global__ void __launch_bounds__(256, FR <= 2 ? 2 : 1) grad_tile_kernel(GradArg
         if (r >= a.m) continue;
 #pragma unroll
         for (int q = 0; q < 8; q++) {
-            const uint64_t k = k0 + q * 16 + (lane >> 4) * 4;
+            const uint64_t k = k0 + q * 16 + g * 4;
             if (k < a.ldp) *reinterpret_cast<f32x4*>(part + r * a.ldp + k) = acc[i][q];
         }
     }
@@ -226,7 +262,7 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const float* __restrict_
         if (k + t < dim) dx[i * lddx + k + t] = (typename Elem<TYPE>::T)s[t];
 }
 
-constexpr uint32_t kMostRows[3] = {3, 5, 4};   // f32, bf16, f16: what a lane's registers hold
+constexpr uint32_t kMostRows[3] = {2, 5, 5};   // f32, bf16, f16: what LDS holds three steps of
 
 struct GradPlan {
     uint32_t fr;
@@ -248,6 +284,8 @@ GradPlan grad_plan(uint64_t m, uint64_t n, uint64_t dim, uint32_t dctype) {
     const uint64_t steps = (n + kStep - 1) / kStep, tiles = g.tiles_m * g.tiles_k;
     uint64_t want = tiles >= resident ? 1 : resident / tiles;
     if (want > (steps + 3) / 4) want = (steps + 3) / 4;
+    const uint64_t most = 0x3FFF0000ull / points8_row_bytes(dim) / kStep, least_slices = (steps + most - 1) / most;   // a slice's codes: less than 1 GiB
+    if (want < least_slices) want = least_slices;
     if (want < 1) want = 1;
     const uint64_t per = (steps + want - 1) / want;
     g.per_slice = per * kStep;
@@ -259,8 +297,8 @@ GradPlan grad_plan(uint64_t m, uint64_t n, uint64_t dim, uint32_t dctype) {
 
 template <int TYPE, int FR>
 void launch_grad(const GradArgs& a, bool vec, unsigned grid, hipStream_t s) {
-    if (vec) hipLaunchKernelGGL((grad_tile_kernel<TYPE, FR, true>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((grad_tile_kernel<TYPE, FR, false>), dim3(grid), dim3(256), 0, s, a);
+    if (vec) hipLaunchKernelGGL((grad_tile_kernel<TYPE, FR, true>), dim3(grid), dim3(256), (grad_lds<TYPE, FR>()), s, a);
+    else hipLaunchKernelGGL((grad_tile_kernel<TYPE, FR, false>), dim3(grid), dim3(256), (grad_lds<TYPE, FR>()), s, a);
 }
 
 }  // namespace
@@ -297,15 +335,15 @@ int32_t ae_points8_product_grad(const ae_points8* p, uint64_t first, uint64_t n,
             const uint64_t tiles = g.tiles_m * g.tiles_k;
             GradArgs a{d_dc, lddc, m, n, p->dim, points8_rows(p, first, n), g.per_slice, (float*)d_work, g.ldp, (uint32_t)g.tiles_k, (uint32_t)tiles, (uint32_t)g.slices};
             const unsigned grid = (unsigned)((tiles * g.slices + 7) / 8 * 8);
-            const bool vec = vector_rows(d_dc, dctype, lddc) && lddc * type_size(dctype) < 0x7FFF0000ull / (64 * g.fr);
+            const bool vec = vector_rows(d_dc, dctype, lddc) && lddc * type_size(dctype) < 0x3FFF0000ull / (64 * g.fr);
             by_type(dctype, [&](auto ty) {
                 constexpr int TYPE = decltype(ty)::value;
                 switch (g.fr) {
                     case 1: launch_grad<TYPE, 1>(a, vec, grid, s); break;
                     case 2: launch_grad<TYPE, 2>(a, vec, grid, s); break;
-                    case 3: launch_grad<TYPE, 3>(a, vec, grid, s); break;
+                    case 3: if constexpr (TYPE != AE_TYPE_F32) launch_grad<TYPE, 3>(a, vec, grid, s); break;
                     case 4: if constexpr (TYPE != AE_TYPE_F32) launch_grad<TYPE, 4>(a, vec, grid, s); break;
-                    default: if constexpr (TYPE == AE_TYPE_BF16) launch_grad<TYPE, 5>(a, vec, grid, s); break;
+                    default: if constexpr (TYPE != AE_TYPE_F32) launch_grad<TYPE, 5>(a, vec, grid, s); break;
                 }
             });
             check_launch("points8_product_grad");

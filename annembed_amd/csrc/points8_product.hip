@@ -74,8 +74,9 @@ struct Walk {
 // Rows: fragment i of a wave's WM rows is rows i, i + FM, i + 2 FM ... of them (FM = WM / 16): the FM rows of a lane are neighbours, their
 // scale bytes one or two dwords, and the matrix cores pick the byte.  The same for the points, so a lane ends up with 16 consecutive
 // columns of each of its rows and writes them itself.
-// LDS: fragment by fragment, a row's 128 codes as 8 chunks of 16 bytes, chunk c of LDS row r at place c ^ ((r >> 1) & 7): 16 lanes that read the
-// same chunk of 16 rows touch all 64 banks once.  The copies to LDS write lane after lane, so the lanes permute what they fetch.
+// LDS: fragment by fragment, a row's 128 codes as 8 chunks of 16 bytes, chunk c of LDS row r at place c ^ ((r >> 1) & 7).  The lanes of group g read
+// chunks g and g + 4: the 16 lanes that LDS serves at a time (0-3, 12-15 and 20-27 of a half wave, then the others) touch all 64 banks once.  (With chunks
+// 2 g and 2 g + 1 two of them meet in every bank.)  The copies to LDS write lane after lane, so the lanes permute what they fetch.
 // Rows beyond the operands and bytes beyond a row lie outside the buffers' range and read as 0.
 //
 // The blocks of all tiles of a workgroup form one stream: the copy runs two blocks ahead of the products, across the end of a tile, and the
@@ -161,16 +162,16 @@ product_tile_kernel(ProductArgs a) {
     };
     i32x8 fx[4], fp[FN];        // of f32 only the first halves
     bf16x8 wp[FN][2];           // f32: the points' values of half a block
-    const int r_x = wi + (lane & 15), r_p = BM + wj + (lane & 15), c0 = (lane >> 4) * 2;
+    const int r_x = wi + (lane & 15), r_p = BM + wj + (lane & 15), c0 = lane >> 4;
     uint32_t in_x = r_x * kBlock + ((c0 ^ ((r_x >> 1) & 7)) << 4), in_p = r_p * kBlock + ((c0 ^ ((r_p >> 1) & 7)) << 4);
     auto chunk_at = [&](uint32_t at) { return *reinterpret_cast<const u32x4*>(lds + at); };
     auto read_x = [&](int s) {
-        if constexpr (EXACT) fx[s & 3] = join(chunk_at((in_x ^ (s / FM * 16)) + s % FM * 16 * kBlock), u32x4{0, 0, 0, 0});
-        else fx[s & 3] = join(chunk_at(in_x + s * 16 * kBlock), chunk_at((in_x ^ 16) + s * 16 * kBlock));
+        if constexpr (EXACT) fx[s & 3] = join(chunk_at((in_x ^ (s / FM * 64)) + s % FM * 16 * kBlock), u32x4{0, 0, 0, 0});
+        else fx[s & 3] = join(chunk_at(in_x + s * 16 * kBlock), chunk_at((in_x ^ 64) + s * 16 * kBlock));
     };
     auto read_p = [&](int j, int h) {
-        if constexpr (EXACT) fp[j] = join(chunk_at((in_p ^ (h * 16)) + j * 16 * kBlock), u32x4{0, 0, 0, 0});
-        else fp[j] = join(chunk_at(in_p + j * 16 * kBlock), chunk_at((in_p ^ 16) + j * 16 * kBlock));
+        if constexpr (EXACT) fp[j] = join(chunk_at((in_p ^ (h * 64)) + j * 16 * kBlock), u32x4{0, 0, 0, 0});
+        else fp[j] = join(chunk_at(in_p + j * 16 * kBlock), chunk_at((in_p ^ 64) + j * 16 * kBlock));
     };
     auto block = [&](uint32_t stage, auto first) {
 #pragma unroll
