@@ -52,9 +52,6 @@ inline Rows8 points8_rows(const ae_points8* p, uint64_t first, uint64_t n) {
 // n rows of x into codes[n][row_bytes] / scales[blocks][scale_stride]
 void points8_quantise(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint8_t* codes, uint8_t* scales, uint64_t scale_stride, hipStream_t s);
 
-// can rows at ptr with this stride be accessed 16 bytes at a time?
-inline bool vector_rows(const void* ptr, uint32_t type, uint64_t ld) { return (uintptr_t)ptr % 16 == 0 && ld * type_size(type) % 16 == 0; }
-
 template <int TYPE> struct Elem;
 template <> struct Elem<AE_TYPE_F32> { using T = float; };
 template <> struct Elem<AE_TYPE_BF16> { using T = __bf16; };
@@ -77,19 +74,16 @@ using i32x8 = __attribute__((ext_vector_type(8))) int;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 
-// eight consecutive elements; `vec`: the address is on 16 bytes and all eight exist, else `count` of them (the others 0)
+// Eight consecutive elements, or `count` of them (the others 0).  Eight are fetched 16 bytes at a time whatever their address: the
+// memory pipeline takes vectors at any alignment, at the price of the lines that they cross.
 template <int TYPE>
-__device__ __forceinline__ void load8(const typename Elem<TYPE>::T* __restrict__ p, bool vec, int count, float (&v)[8]) {
+__device__ __forceinline__ void load8(const typename Elem<TYPE>::T* __restrict__ p, int count, float (&v)[8]) {
     using T = typename Elem<TYPE>::T;
-    if (vec) {
-        constexpr int W = 16 / sizeof(T);
-        using V = __attribute__((ext_vector_type(W))) T;
+    if (count == 8) {
+        T a[8];
+        __builtin_memcpy(a, p, sizeof(a));
 #pragma unroll
-        for (int q = 0; q < 8 / W; q++) {
-            const V a = reinterpret_cast<const V*>(p)[q];
-#pragma unroll
-            for (int t = 0; t < W; t++) v[q * W + t] = (float)a[t];
-        }
+        for (int t = 0; t < 8; t++) v[t] = (float)a[t];
     } else {
 #pragma unroll
         for (int t = 0; t < 8; t++) v[t] = t < count ? (float)p[t] : 0.f;
@@ -97,22 +91,16 @@ __device__ __forceinline__ void load8(const typename Elem<TYPE>::T* __restrict__
 }
 // one rounding, to nearest even, where T is narrower than f32
 template <int TYPE>
-__device__ __forceinline__ void store8(typename Elem<TYPE>::T* __restrict__ p, bool vec, int count, const float (&v)[8]) {
+__device__ __forceinline__ void store8(typename Elem<TYPE>::T* __restrict__ p, int count, const float (&v)[8]) {
     using T = typename Elem<TYPE>::T;
-    if (vec) {
-        constexpr int W = 16 / sizeof(T);
-        using V = __attribute__((ext_vector_type(W))) T;
+    T a[8];
 #pragma unroll
-        for (int q = 0; q < 8 / W; q++) {
-            V a;
-#pragma unroll
-            for (int t = 0; t < W; t++) a[t] = (T)v[q * W + t];
-            reinterpret_cast<V*>(p)[q] = a;
-        }
-    } else {
+    for (int t = 0; t < 8; t++) a[t] = (T)v[t];
+    if (count == 8) __builtin_memcpy(p, a, sizeof(a));
+    else {
 #pragma unroll
         for (int t = 0; t < 8; t++)
-            if (t < count) p[t] = (T)v[t];
+            if (t < count) p[t] = a[t];
     }
 }
 

@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(256) points8_release_kernel(const uint32_t* __
 }
 
 // SLOTS 0: row i to first + i.  1: to slots[i], each row scans for a later row of the same slot.  2: to slots[i] where owner says so.
-template <int TYPE, bool VEC, int SLOTS>
+template <int TYPE, int SLOTS>
 __global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<TYPE>::T* __restrict__ x, uint64_t ldx, uint64_t dim, Blocks bl, uint64_t first,
                                                             const uint32_t* __restrict__ slots, const uint32_t* __restrict__ owner, uint64_t capacity,
                                                             uint8_t* __restrict__ codes, uint64_t row_bytes, uint8_t* __restrict__ scales, uint64_t scale_stride) {
@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<
         live[t] = u0 + off < bl.units;
         const uint64_t k = b[t] * (uint64_t)kBlock + lane * 8;
         const int count = !live[t] || k >= dim ? 0 : (int)min((uint64_t)8, dim - k);
-        load8<TYPE>(x + (count ? row[t] * ldx + k : 0), VEC && count == 8, count, v[t]);
+        load8<TYPE>(x + (count ? row[t] * ldx + k : 0), count, v[t]);
     }
 #pragma unroll
     for (int t = 0; t < kTrips; t++) {
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<
     }
 }
 
-template <int TYPE, bool VEC, bool SLOTS>
+template <int TYPE, bool SLOTS>
 __global__ void __launch_bounds__(256) points8_read_kernel(const uint8_t* __restrict__ codes, uint64_t row_bytes, const uint8_t* __restrict__ scales, uint64_t scale_stride,
                                                            uint64_t capacity, uint64_t first, const uint32_t* __restrict__ slots, Blocks bl,
                                                            typename Elem<TYPE>::T* __restrict__ x, uint64_t ldx, uint64_t dim) {
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256) points8_read_kernel(const uint8_t* __rest
             for (int q = 0; q < 8; q++) v[q] = __uint_as_float(0x7FC00000u);
         }
         const uint64_t k = b[t] * (uint64_t)kBlock + lane * 8;
-        if (count[t]) store8<TYPE>(x + row[t] * ldx + k, VEC && count[t] == 8, count[t], v);
+        if (count[t]) store8<TYPE>(x + row[t] * ldx + k, count[t], v);
     }
 }
 
@@ -161,11 +161,8 @@ void launch_write(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint
     by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         const auto* x = static_cast<const typename Elem<TYPE>::T*>(d_x);
-        auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales, scale_stride);
-        };
-        if (vector_rows(d_x, type, ldx)) go(points8_write_kernel<TYPE, true, SLOTS>);
-        else go(points8_write_kernel<TYPE, false, SLOTS>);
+        hipLaunchKernelGGL((points8_write_kernel<TYPE, SLOTS>), dim3(grid), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales,
+                           scale_stride);
     });
     check_launch("points8_write");
 }
@@ -180,9 +177,8 @@ void read_rows(const ae_points8* p, uint64_t first, const uint32_t* slots, uint6
             hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, (const uint8_t*)p->codes.p, p->row_bytes, (const uint8_t*)p->scales.p, p->scale_stride, p->capacity, first,
                                slots, bl, x, ldx, p->dim);
         };
-        const bool vec = vector_rows(d_x, type, ldx);
-        if (slots) { if (vec) go(points8_read_kernel<TYPE, true, true>); else go(points8_read_kernel<TYPE, false, true>); }
-        else { if (vec) go(points8_read_kernel<TYPE, true, false>); else go(points8_read_kernel<TYPE, false, false>); }
+        if (slots) go(points8_read_kernel<TYPE, true>);
+        else go(points8_read_kernel<TYPE, false>);
     });
     check_launch("points8_read");
 }

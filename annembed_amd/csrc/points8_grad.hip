@@ -11,8 +11,6 @@
 // bytes.  One barrier a step.  Few rows leave few tiles: the points are split into slices whose sums are joined in order.
 #include "points8.h"
 
-#include <algorithm>
-
 using namespace ae;
 
 namespace {
@@ -62,10 +60,10 @@ struct GradArgs {
     uint32_t tiles_k, tiles, slices;
 };
 
-template <int TYPE, int FR> constexpr int grad_lds() { return 3 * 64 * FR * kStep * (TYPE == AE_TYPE_F32 ? 4 : 2) + 2 * kBlock * 128; }
+template <int TYPE, int FR> constexpr int grad_lds() { return 3 * 64 * FR * kStep * (TYPE == AE_TYPE_F32 ? 4 : 2) + 2 * kBlock * 128; }   // 56 or 80 KB: two workgroups a CU
 
-template <int TYPE, int FR, bool VEC>   // VEC: rows of dc lie on 16 bytes, 64 FR of them span less than 1 GiB
-__global__ void __launch_bounds__(256, (grad_lds<TYPE, FR>() <= 80 * 1024 ? 2 : 1)) grad_tile_kernel(GradArgs a) {
+template <int TYPE, int FR, bool VEC>   // VEC: the copies' 32-bit offsets and whole pieces do for dc
+__global__ void __launch_bounds__(256, 2) grad_tile_kernel(GradArgs a) {
     using T = typename Elem<TYPE>::T;
     constexpr int TERMS = terms_of<TYPE>(), ROW = kStep * (int)sizeof(T), PIECES = ROW / 16, STAGE = 64 * FR * ROW, COPIES = STAGE / 4096;
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];   // three stages of dc, two of coordinates
@@ -81,11 +79,11 @@ __global__ void __launch_bounds__(256, (grad_lds<TYPE, FR>() <= 80 * 1024 ? 2 : 
     const uint32_t mi = (uint32_t)min((uint64_t)(64 * FR), a.m - i0), points = (uint32_t)(je - jb), steps = (points + kStep - 1) / kStep;
     const int r0 = wave * 16 * FR + (lane & 15);   // this lane's first row of the tile; the others 16 apart
     const T* dc = static_cast<const T*>(a.dc) + i0 * a.lddc + jb;
-    // Rows beyond m lie outside the buffer's range, which ends with the piece of the last row's last point: it is fetched whole (it lies on
-    // 16 bytes, so in one page).  A lane's offsets never change, the step goes into the scalar one, which stays inside the range (steps past the
-    // last one fetch the last again, for nobody).  What is fetched behind the last point is cut in the last step.
+    // Rows beyond m lie outside the buffer's range, which ends with the dword of the last row's last point (what of a piece lies behind it reads as
+    // 0).  A lane's offsets never change, the step goes into the scalar one, which stays inside the range (steps past the last one fetch the last
+    // again, for nobody).  What is fetched behind the last point is cut in the last step.
     const uint32_t row_bytes = (uint32_t)a.lddc * (uint32_t)sizeof(T);
-    __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)dc, (short)0, VEC ? (int)((mi - 1) * row_bytes + (points * (uint32_t)sizeof(T) + 15) / 16 * 16) : 0, 0x00027000);
+    __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)dc, (short)0, VEC ? (int)((mi - 1) * row_bytes + (points * (uint32_t)sizeof(T) + 3) / 4 * 4) : 0, 0x00027000);
     __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.codes + jb * a.p.row_bytes), (short)0, (int)(points * (uint32_t)a.p.row_bytes), 0x00027000);
     const uint32_t k_at = (uint32_t)k0 + kg * 4, code_at = (uint32_t)(jg * 8) * (uint32_t)a.p.row_bytes + (k_at < a.p.row_bytes ? k_at : kOutside);
     const uint8_t* sc = a.p.scales + tk * a.p.scale_stride + jb + jg * 8;
@@ -262,25 +260,18 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const float* __restrict_
         if (k + t < dim) dx[i * lddx + k + t] = (typename Elem<TYPE>::T)s[t];
 }
 
-constexpr uint32_t kMostRows[3] = {2, 5, 5};   // f32, bf16, f16: what LDS holds three steps of
-
 struct GradPlan {
     uint32_t fr;
     uint64_t tiles_m, tiles_k, slices, per_slice, ldp, bytes;
 };
 GradPlan grad_plan(uint64_t m, uint64_t n, uint64_t dim, uint32_t dctype) {
     GradPlan g;
-    const char* v = debug_knob("AE_P8G");
-    uint32_t best = 1;
-    uint64_t least = ~0ull;
-    for (uint32_t fr = 1; fr <= kMostRows[dctype]; fr++) {
-        const uint64_t padded = (m + 64 * fr - 1) / (64 * fr) * (64 * fr);
-        if (padded <= least) { least = padded; best = fr; }
-    }
-    g.fr = v ? std::min<uint32_t>(atoi(v), kMostRows[dctype]) : best;
+    // 128 rows read the points half as often as 64 (300 x 60 000 x 784 of bf16: 52 against 67 us, 1024 rows: 127 against 189); more of them, or 128 of
+    // f32, leave one workgroup on a CU, whose waits nothing fills (256 rows: 73 and 135 us; f32, 128 rows: 165 against 116 us)
+    g.fr = m > 64 && dctype != AE_TYPE_F32 ? 2 : 1;
     g.tiles_m = (m + 64 * g.fr - 1) / (64 * g.fr);
     g.tiles_k = (dim + kBlock - 1) / kBlock;
-    const uint64_t resident = g.fr <= 2 ? 512 : 256;
+    const uint64_t resident = 512;   // two workgroups on each of 256 CUs
     const uint64_t steps = (n + kStep - 1) / kStep, tiles = g.tiles_m * g.tiles_k;
     uint64_t want = tiles >= resident ? 1 : resident / tiles;
     if (want > (steps + 3) / 4) want = (steps + 3) / 4;
@@ -335,16 +326,14 @@ int32_t ae_points8_product_grad(const ae_points8* p, uint64_t first, uint64_t n,
             const uint64_t tiles = g.tiles_m * g.tiles_k;
             GradArgs a{d_dc, lddc, m, n, p->dim, points8_rows(p, first, n), g.per_slice, (float*)d_work, g.ldp, (uint32_t)g.tiles_k, (uint32_t)tiles, (uint32_t)g.slices};
             const unsigned grid = (unsigned)((tiles * g.slices + 7) / 8 * 8);
-            const bool vec = vector_rows(d_dc, dctype, lddc) && lddc * type_size(dctype) < 0x3FFF0000ull / (64 * g.fr);
+            // The copies take 16 bytes at any address and the dwords that the buffer's range holds whole.  The last of an odd number of 16-bit values is the
+            // first half of a dword: the range then goes 2 bytes past it, which must not be the next page.
+            const uint64_t size = type_size(dctype), end = (uint64_t)(uintptr_t)d_dc + ((m - 1) * lddc + n) * size;
+            const bool vec = lddc * size < 0x3FFF0000ull / (64 * g.fr) && (n * size % 4 == 0 || end % 4096 != 0);
             by_type(dctype, [&](auto ty) {
                 constexpr int TYPE = decltype(ty)::value;
-                switch (g.fr) {
-                    case 1: launch_grad<TYPE, 1>(a, vec, grid, s); break;
-                    case 2: launch_grad<TYPE, 2>(a, vec, grid, s); break;
-                    case 3: if constexpr (TYPE != AE_TYPE_F32) launch_grad<TYPE, 3>(a, vec, grid, s); break;
-                    case 4: if constexpr (TYPE != AE_TYPE_F32) launch_grad<TYPE, 4>(a, vec, grid, s); break;
-                    default: if constexpr (TYPE != AE_TYPE_F32) launch_grad<TYPE, 5>(a, vec, grid, s); break;
-                }
+                if (g.fr == 1) launch_grad<TYPE, 1>(a, vec, grid, s);
+                else if constexpr (TYPE != AE_TYPE_F32) launch_grad<TYPE, 2>(a, vec, grid, s);
             });
             check_launch("points8_product_grad");
         }

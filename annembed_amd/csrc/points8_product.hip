@@ -45,7 +45,7 @@ struct ProductArgs {
     void* c;
     uint64_t ldc;
     uint32_t tiles_m, tiles_n;
-    uint32_t vec;     // rows of c can be written 16 bytes at a time, and a tile's rows span less than 2 GiB
+    uint32_t near;    // a tile's rows of c span less than 2 GiB
 };
 
 // The tiles of a workgroup.  Workgroups go to the 8 XCDs in turn, each with an L2 of its own: an XCD owns a run of the tiles, kPanel rows of
@@ -277,7 +277,7 @@ product_tile_kernel(ProductArgs a) {
         const int mi = (int)min((uint64_t)BM, a.x.rows - i0), nj = (int)min((uint64_t)BN, a.p.rows - j0);
         constexpr int W = 16 / sizeof(T);
         const int row = wi + (lane & 15) * FM, col = wj + (lane >> 4) * 16;
-        if (a.vec && (nj == BN || nj % W == 0)) {
+        if (a.near && (nj == BN || nj % W == 0)) {
             __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)c, (short)0, (int)(((uint32_t)(mi - 1) * (uint32_t)a.ldc + (uint32_t)nj) * (uint32_t)sizeof(T)), 0x00027000);
             // the four lanes of a row change 16-byte pieces among them, so that a store writes 64 consecutive bytes of 16 rows
             const int piece = wj + (lane >> 4) * W;
@@ -319,8 +319,8 @@ void launch_tiles(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint3
     const uint64_t tiles_m = (x.rows + BM - 1) / BM, tiles_n = (p.rows + BN - 1) / BN, tiles = tiles_m * tiles_n;
     if (tiles > 0x3FFFFFFFull) fail(AE_ERR_INVALID_ARG, "ae_points8_product: %llu x %llu are more products than one call takes", (unsigned long long)x.rows, (unsigned long long)p.rows);
     constexpr unsigned threads = (BM / WM) * (BN / 64) * 64, bytes = 2 * (BM + BN) * kBlock, resident = 256 * (bytes > 80 * 1024 ? 1 : 2);
-    const bool vec = vector_rows(d_c, ctype, ldc) && ldc * type_size(ctype) < 0x7FFF0000ull / BM;
-    const ProductArgs a{x, p, points8_blocks(dim), d_c, ldc, (uint32_t)tiles_m, (uint32_t)tiles_n, vec ? 1u : 0u};
+    const bool near = ldc * type_size(ctype) < 0x7FFF0000ull / BM;
+    const ProductArgs a{x, p, points8_blocks(dim), d_c, ldc, (uint32_t)tiles_m, (uint32_t)tiles_n, near ? 1u : 0u};
     const unsigned grid = tiles < resident ? (unsigned)((tiles + 7) / 8 * 8) : resident;
     by_type(ctype, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;

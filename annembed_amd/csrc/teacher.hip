@@ -84,9 +84,9 @@ __device__ __forceinline__ double take_list(const TeacherList& t, uint64_t r, ui
 
 // One workgroup per row.  LOSS: statistics, loss and (grad not null) the gradient; otherwise the gradient from kept statistics.
 template <int TYPE, bool LOSS>
-__global__ void __launch_bounds__(256) teacher_row_kernel(const typename Elem<TYPE>::T* __restrict__ logits_, uint64_t cols, uint64_t ld, bool vec, TeacherList list,
+__global__ void __launch_bounds__(256) teacher_row_kernel(const typename Elem<TYPE>::T* __restrict__ logits_, uint64_t cols, uint64_t ld, TeacherList list,
                                                           float temperature, const float* __restrict__ weight, float* __restrict__ loss, float* stats,
-                                                          typename Elem<TYPE>::T* grad_, uint64_t ldg, bool vecg) {
+                                                          typename Elem<TYPE>::T* grad_, uint64_t ldg) {
     using T = typename Elem<TYPE>::T;
     __shared__ uint32_t li[kMaxList];
     __shared__ float lp[kMaxList];
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256) teacher_row_kernel(const typename Elem<TY
             for (uint64_t v0 = (uint64_t)tid * 8; v0 < cols; v0 += 256 * 8) {
                 const int count = (int)min((uint64_t)8, cols - v0);
                 float v[8];
-                load8<TYPE>(row + v0, vec && count == 8, count, v);
+                load8<TYPE>(row + v0, count, v);
                 float big = -INFINITY;
 #pragma unroll
                 for (int t = 0; t < 8; t++) {
@@ -170,11 +170,11 @@ __global__ void __launch_bounds__(256) teacher_row_kernel(const typename Elem<TY
 #pragma unroll
             for (int t = 0; t < 8; t++) v[t] = 0.f;
         } else {
-            load8<TYPE>(row + v0, vec && count == 8, count, v);
+            load8<TYPE>(row + v0, count, v);
 #pragma unroll
             for (int t = 0; t < 8; t++) v[t] = g * (p_sum * __builtin_amdgcn_exp2f((v[t] - m) * c + lift));
         }
-        store8<TYPE>(grow + v0, vecg && count == 8, count, v);
+        store8<TYPE>(grow + v0, count, v);
     }
     if (out) return;
     // the listed columns again, with their probabilities: after every store of the row has left this CU
@@ -207,8 +207,8 @@ void launch_rows(const void* d_logits, uint32_t type, uint64_t rows, uint64_t co
     by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         using T = typename Elem<TYPE>::T;
-        hipLaunchKernelGGL((teacher_row_kernel<TYPE, LOSS>), dim3((unsigned)rows), dim3(256), 0, s, static_cast<const T*>(d_logits), cols, ld, vector_rows(d_logits, type, ld), list,
-                           temperature, weight, loss, stats, static_cast<T*>(d_grad), ldg, d_grad && vector_rows(d_grad, type, ldg));
+        hipLaunchKernelGGL((teacher_row_kernel<TYPE, LOSS>), dim3((unsigned)rows), dim3(256), 0, s, static_cast<const T*>(d_logits), cols, ld, list,
+                           temperature, weight, loss, stats, static_cast<T*>(d_grad), ldg);
     });
     check_launch("teacher_row");
 }
