@@ -74,16 +74,22 @@ using i32x8 = __attribute__((ext_vector_type(8))) int;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 
-// Eight consecutive elements, or `count` of them (the others 0).  Eight are fetched 16 bytes at a time whatever their address: the
-// memory pipeline takes vectors at any alignment, at the price of the lines that they cross.
+// 16 bytes at any address of a 16-bit element: the memory pipeline takes vectors at any alignment, at the price of the lines that they cross
+typedef uint32_t Piece __attribute__((ext_vector_type(4), aligned(2)));
+
+// eight consecutive elements, or `count` of them (the others 0)
 template <int TYPE>
 __device__ __forceinline__ void load8(const typename Elem<TYPE>::T* __restrict__ p, int count, float (&v)[8]) {
     using T = typename Elem<TYPE>::T;
+    constexpr int W = 16 / sizeof(T);
+    using V = __attribute__((ext_vector_type(W))) T;
     if (count == 8) {
-        T a[8];
-        __builtin_memcpy(a, p, sizeof(a));
 #pragma unroll
-        for (int t = 0; t < 8; t++) v[t] = (float)a[t];
+        for (int q = 0; q < 8 / W; q++) {
+            const V a = __builtin_bit_cast(V, reinterpret_cast<const Piece*>(p)[q]);
+#pragma unroll
+            for (int t = 0; t < W; t++) v[q * W + t] = (float)a[t];
+        }
     } else {
 #pragma unroll
         for (int t = 0; t < 8; t++) v[t] = t < count ? (float)p[t] : 0.f;
@@ -93,14 +99,20 @@ __device__ __forceinline__ void load8(const typename Elem<TYPE>::T* __restrict__
 template <int TYPE>
 __device__ __forceinline__ void store8(typename Elem<TYPE>::T* __restrict__ p, int count, const float (&v)[8]) {
     using T = typename Elem<TYPE>::T;
-    T a[8];
+    constexpr int W = 16 / sizeof(T);
+    using V = __attribute__((ext_vector_type(W))) T;
+    if (count == 8) {
 #pragma unroll
-    for (int t = 0; t < 8; t++) a[t] = (T)v[t];
-    if (count == 8) __builtin_memcpy(p, a, sizeof(a));
-    else {
+        for (int q = 0; q < 8 / W; q++) {
+            V a;
+#pragma unroll
+            for (int t = 0; t < W; t++) a[t] = (T)v[q * W + t];
+            reinterpret_cast<Piece*>(p)[q] = __builtin_bit_cast(Piece, a);
+        }
+    } else {
 #pragma unroll
         for (int t = 0; t < 8; t++)
-            if (t < count) p[t] = a[t];
+            if (t < count) p[t] = (T)v[t];
     }
 }
 

@@ -82,41 +82,118 @@ __device__ __forceinline__ double take_list(const TeacherList& t, uint64_t r, ui
     return __ballot(outside) ? (double)__uint_as_float(0x7FC00000u) : p_sum;
 }
 
-// One workgroup per row.  LOSS: statistics, loss and (grad not null) the gradient; otherwise the gradient from kept statistics.
-template <int TYPE, bool LOSS>
-__global__ void __launch_bounds__(256) teacher_row_kernel(const typename Elem<TYPE>::T* __restrict__ logits_, uint64_t cols, uint64_t ld, TeacherList list,
-                                                          float temperature, const float* __restrict__ weight, float* __restrict__ loss, float* stats,
-                                                          typename Elem<TYPE>::T* grad_, uint64_t ldg) {
+// Elements of a row in pieces of 16 bytes; `count` of the piece's exist
+template <int TYPE> constexpr int piece_len() { return 16 / (int)sizeof(typename Elem<TYPE>::T); }
+template <int TYPE>
+__device__ __forceinline__ Piece load_piece(const typename Elem<TYPE>::T* p, int64_t count) {
     using T = typename Elem<TYPE>::T;
+    constexpr int W = piece_len<TYPE>();
+    if (count >= W) return *reinterpret_cast<const Piece*>(p);
+    using V = __attribute__((ext_vector_type(W))) T;
+    V v;
+#pragma unroll
+    for (int t = 0; t < W; t++) v[t] = t < count ? p[t] : (T)-INFINITY;   // (an exponential of 0, never the largest)
+    return __builtin_bit_cast(Piece, v);
+}
+template <int TYPE>
+__device__ __forceinline__ void store_piece(typename Elem<TYPE>::T* p, int64_t count, const float (&x)[16 / sizeof(typename Elem<TYPE>::T)]) {
+    using T = typename Elem<TYPE>::T;
+    constexpr int W = piece_len<TYPE>();
+    using V = __attribute__((ext_vector_type(W))) T;
+    V v;
+#pragma unroll
+    for (int t = 0; t < W; t++) v[t] = (T)x[t];
+    if (count >= W) *reinterpret_cast<Piece*>(p) = __builtin_bit_cast(Piece, v);
+    else {
+#pragma unroll
+        for (int t = 0; t < W; t++)
+            if (t < count) p[t] = v[t];
+    }
+}
+
+// One workgroup of THREADS per row.  HELD pieces of 16 bytes a thread hold the whole row in registers: it is read once, whatever is made of it.
+// HELD 0: longer rows are read again for the gradient, mostly from the caches.  LOSS: statistics, loss and (grad not null) the gradient;
+// otherwise the gradient from kept statistics.
+template <int TYPE, int THREADS, int HELD, bool LOSS>
+__global__ void __launch_bounds__(THREADS) teacher_row_kernel(const typename Elem<TYPE>::T* logits_, uint64_t cols, uint64_t ld, TeacherList list, float temperature,
+                                                              const float* __restrict__ weight, float* __restrict__ loss, float* stats, typename Elem<TYPE>::T* grad_, uint64_t ldg) {
+    using T = typename Elem<TYPE>::T;
+    constexpr int W = piece_len<TYPE>(), WAVES = THREADS / 64;
+    using V = __attribute__((ext_vector_type(W))) T;
     __shared__ uint32_t li[kMaxList];
-    __shared__ float lp[kMaxList];
-    __shared__ float ls[kMaxList];
-    __shared__ float sm[4], ss[4];
-    __shared__ double sd[1];
+    __shared__ float lp[kMaxList], ls[kMaxList];
+    __shared__ float sm[WAVES], ss[WAVES];
+    __shared__ double sd[2];
     const uint64_t r = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const T* row = logits_ + r * ld;
     T* grow = grad_ ? grad_ + r * ldg : nullptr;
     const float w = weight ? weight[r] : 1.f;
     const float c = kLog2e / temperature;
-    float m = -INFINITY, lnsum = 0.f;
-    if (w != 0.f) {
+    const bool counts = w != 0.f && (LOSS || stats[2 * r] != -INFINITY);
+    if (!counts) {   // the row is left out
         if constexpr (LOSS) {
-            Running run;
-            for (uint64_t v0 = (uint64_t)tid * 8; v0 < cols; v0 += 256 * 8) {
-                const int count = (int)min((uint64_t)8, cols - v0);
-                float v[8];
-                load8<TYPE>(row + v0, count, v);
-                float big = -INFINITY;
+            if (tid == 0) { stats[2 * r] = -INFINITY; stats[2 * r + 1] = 0.f; loss[r] = 0.f; }
+        }
+        if (grow) {
+            const float zero[W] = {};
+            for (uint64_t v0 = (uint64_t)tid * W; v0 < cols; v0 += THREADS * W) store_piece<TYPE>(grow + v0, (int64_t)(cols - v0), zero);
+        }
+        return;
+    }
+    // The list, by the first wave, before its part of the row: its 64-bit logarithms and the row would not fit in the registers together, and the other
+    // waves and rows of the CU go on meanwhile.
+    double plogp = 0.;
+    if (wave == 0) {
+        const double p = take_list(list, r, cols, temperature, li, lp, plogp);
+        for (uint32_t j = lane; j < list.k; j += 64) ls[j] = li[j] == 0xFFFFFFFFu ? 0.f : (float)row[li[j]];   // (a lane reads back what it wrote)
+        if (lane == 0) sd[0] = p;
+    }
+    Piece held[HELD ? HELD : 1];
+    if constexpr (HELD) {
 #pragma unroll
-                for (int t = 0; t < 8; t++) {
-                    if (t >= count) v[t] = -INFINITY;
-                    big = fmaxf(big, v[t]);
-                }
+        for (int q = 0; q < HELD; q++) {
+            const int64_t v0 = (int64_t)(q * THREADS + tid) * W, count = (int64_t)cols - v0;
+            if (count > 0) held[q] = load_piece<TYPE>(row + v0, count);
+            else {
+                V none;
+#pragma unroll
+                for (int t = 0; t < W; t++) none[t] = (T)-INFINITY;
+                held[q] = __builtin_bit_cast(Piece, none);
+            }
+        }
+    }
+    float m, lnsum;
+    if constexpr (LOSS) {
+        Running run;
+        if constexpr (HELD) {
+            // largest and sum of the wave
+            float big = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < HELD; q++) {
+                const V v = __builtin_bit_cast(V, held[q]);
+#pragma unroll
+                for (int t = 0; t < W; t++) big = fmaxf(big, (float)v[t]);
+            }
+            run.m = wave_max(big);
+            const float safe = run.m == -INFINITY ? 0.f : run.m;
+#pragma unroll
+            for (int q = 0; q < HELD; q++) {
+                const V v = __builtin_bit_cast(V, held[q]);
+#pragma unroll
+                for (int t = 0; t < W; t++) run.s += __builtin_amdgcn_exp2f(((float)v[t] - safe) * c);
+            }
+#pragma unroll
+            for (int o = 32; o; o >>= 1) run.s += __shfl_xor(run.s, o);
+        } else {
+            for (uint64_t v0 = (uint64_t)tid * W; v0 < cols; v0 += THREADS * W) {
+                const V v = __builtin_bit_cast(V, load_piece<TYPE>(row + v0, (int64_t)(cols - v0)));
+                float big = -INFINITY, s = 0.f;
+#pragma unroll
+                for (int t = 0; t < W; t++) big = fmaxf(big, (float)v[t]);
                 const float safe = big == -INFINITY ? 0.f : big;
-                float s = 0.f;
 #pragma unroll
-                for (int t = 0; t < 8; t++) s += __builtin_amdgcn_exp2f((v[t] - safe) * c);
+                for (int t = 0; t < W; t++) s += __builtin_amdgcn_exp2f(((float)v[t] - safe) * c);
                 run.join(big, s, c);
             }
 #pragma unroll
@@ -124,68 +201,64 @@ __global__ void __launch_bounds__(256) teacher_row_kernel(const typename Elem<TY
                 const float m2 = __shfl_xor(run.m, o), s2 = __shfl_xor(run.s, o);
                 run.join(m2, s2, c);
             }
-            if (lane == 0) { sm[wave] = run.m; ss[wave] = run.s; }
-            __syncthreads();
-            run = Running();
-#pragma unroll
-            for (int q = 0; q < 4; q++) run.join(sm[q], ss[q], c);
-            m = run.m;
-            if (run.s != run.s) m = run.s;   // a NaN or +inf among the logits
-            lnsum = m == -INFINITY ? 0.f : (float)log((double)run.s);
-        } else {
-            m = stats[2 * r];
-            lnsum = stats[2 * r + 1];
         }
-    }
-    const bool out = m == -INFINITY;   // weight 0, or nothing but -inf: the row is left out
-    if constexpr (LOSS) {
+        if (lane == 0) { sm[wave] = run.m; ss[wave] = run.s; }
+        __syncthreads();
+        run = Running();
+#pragma unroll
+        for (int q = 0; q < WAVES; q++) run.join(sm[q], ss[q], c);
+        m = run.s != run.s ? run.s : run.m;   // NaN: a NaN or +inf among the logits
+        lnsum = m == -INFINITY ? 0.f : (float)log((double)run.s);
         if (tid == 0) { stats[2 * r] = m; stats[2 * r + 1] = lnsum; }
+    } else {
+        m = stats[2 * r];
+        lnsum = stats[2 * r + 1];
+        __syncthreads();   // (the list)
     }
-    if (!out && wave == 0) {
-        double plogp = 0.;
-        const double p = take_list(list, r, cols, temperature, li, lp, plogp);
-        double cross = 0.;
-        for (uint32_t j = lane; j < list.k; j += 64) {   // (a lane reads back what it wrote)
-            const uint32_t v = li[j];
-            const float s = v == 0xFFFFFFFFu ? 0.f : (float)row[v];
-            ls[j] = s;
-            if (lp[j] != 0.f) cross += (double)lp[j] * (((double)s - (double)m) / (double)temperature - (double)lnsum);
-        }
-        cross = wave_sum(cross);
-        if (lane == 0) {
-            sd[0] = p;
-            if constexpr (LOSS) loss[r] = (p != p || m != m) ? __uint_as_float(0x7FC00000u) : (float)((double)w * (plogp - cross));
+    const bool out = LOSS && m == -INFINITY;   // nothing but -inf
+    if constexpr (LOSS) {
+        if (wave == 0) {
+            double cross = 0.;
+            if (!out)
+                for (uint32_t j = lane; j < list.k; j += 64)
+                    if (lp[j] != 0.f) cross += (double)lp[j] * (((double)ls[j] - (double)m) / (double)temperature - (double)lnsum);
+            cross = wave_sum(cross);
+            if (lane == 0) loss[r] = out ? 0.f : (sd[0] != sd[0] || m != m) ? __uint_as_float(0x7FC00000u) : (float)((double)w * (plogp - cross));
         }
     }
-    if constexpr (LOSS) { if (out && tid == 0) loss[r] = 0.f; }
     if (!grow) return;
-    __syncthreads();
-    const float g = out ? 0.f : w / temperature;
-    const float p_sum = out ? 0.f : (float)sd[0];
-    const float lift = -lnsum * kLog2e;
-    for (uint64_t v0 = (uint64_t)tid * 8; v0 < cols; v0 += 256 * 8) {
-        const int count = (int)min((uint64_t)8, cols - v0);
-        float v[8];
-        if (out) {
+    const float g = out ? 0.f : w / temperature, p_sum = out ? 0.f : (float)sd[0], lift = -lnsum * kLog2e, base = out ? 0.f : m;
+    auto gradient = [&](float v) { return out ? 0.f : g * (p_sum * __builtin_amdgcn_exp2f((v - base) * c + lift)); };
+    // in place: the listed logits have been taken by the first wave before the barrier
+    if constexpr (HELD) {
 #pragma unroll
-            for (int t = 0; t < 8; t++) v[t] = 0.f;
-        } else {
-            load8<TYPE>(row + v0, count, v);
+        for (int q = 0; q < HELD; q++) {
+            const int64_t v0 = (int64_t)(q * THREADS + tid) * W, count = (int64_t)cols - v0;
+            if (count <= 0) continue;
+            const V v = __builtin_bit_cast(V, held[q]);
+            float x[W];
 #pragma unroll
-            for (int t = 0; t < 8; t++) v[t] = g * (p_sum * __builtin_amdgcn_exp2f((v[t] - m) * c + lift));
+            for (int t = 0; t < W; t++) x[t] = gradient((float)v[t]);
+            store_piece<TYPE>(grow + v0, count, x);
         }
-        store8<TYPE>(grow + v0, count, v);
+    } else {
+        for (uint64_t v0 = (uint64_t)tid * W; v0 < cols; v0 += THREADS * W) {
+            const V v = __builtin_bit_cast(V, load_piece<TYPE>(row + v0, (int64_t)(cols - v0)));
+            float x[W];
+#pragma unroll
+            for (int t = 0; t < W; t++) x[t] = gradient((float)v[t]);
+            store_piece<TYPE>(grow + v0, (int64_t)(cols - v0), x);
+        }
     }
     if (out) return;
-    // the listed columns again, with their probabilities: after every store of the row has left this CU
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (uint32_t j = tid; j < list.k; j += 256) {
+    // The listed columns again, with their probabilities, each by the wave that wrote it above: the stores of a wave to one address stay in
+    // order, nobody waits.
+    for (uint32_t j = lane; j < list.k; j += 64) {
         const uint32_t v = li[j];
-        if (v == 0xFFFFFFFFu) continue;
+        if (v == 0xFFFFFFFFu || (int)(v / W % THREADS / 64) != wave) continue;
         float p = 0.f;
         for (uint32_t o = 0; o < list.k; o++) p += li[o] == v ? lp[o] : 0.f;   // equal columns: the same sum in the same order
-        grow[v] = (T)(g * (p_sum * __builtin_amdgcn_exp2f((ls[j] - m) * c + lift) - p));
+        grow[v] = (T)(g * (p_sum * __builtin_amdgcn_exp2f((ls[j] - base) * c + lift) - p));
     }
 }
 
@@ -207,8 +280,21 @@ void launch_rows(const void* d_logits, uint32_t type, uint64_t rows, uint64_t co
     by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         using T = typename Elem<TYPE>::T;
-        hipLaunchKernelGGL((teacher_row_kernel<TYPE, LOSS>), dim3((unsigned)rows), dim3(256), 0, s, static_cast<const T*>(d_logits), cols, ld, list,
-                           temperature, weight, loss, stats, static_cast<T*>(d_grad), ldg);
+        auto go = [&](auto kernel, unsigned threads) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 0, s, static_cast<const T*>(d_logits), cols, ld, list, temperature, weight, loss, stats,
+                               static_cast<T*>(d_grad), ldg);
+        };
+        // as few threads as hold the row: the more rows a CU has at work, the better their phases mix
+        const uint64_t pieces = (cols + piece_len<TYPE>() - 1) / piece_len<TYPE>();
+        if (pieces <= 64) go(teacher_row_kernel<TYPE, 64, 1, LOSS>, 64);
+        else if (pieces <= 256) go(teacher_row_kernel<TYPE, 256, 1, LOSS>, 256);
+        else if (pieces <= 512) go(teacher_row_kernel<TYPE, 256, 2, LOSS>, 256);
+        else if (pieces <= 1024) go(teacher_row_kernel<TYPE, 256, 4, LOSS>, 256);
+        else if (pieces <= 2048) go(teacher_row_kernel<TYPE, 256, 8, LOSS>, 256);
+        else if (pieces <= 4096) go(teacher_row_kernel<TYPE, 512, 8, LOSS>, 512);
+        else if (pieces <= 8192) go(teacher_row_kernel<TYPE, 1024, 8, LOSS>, 1024);
+        else if (TYPE == AE_TYPE_F32 && pieces <= 16384) go(teacher_row_kernel<TYPE, 1024, TYPE == AE_TYPE_F32 ? 16 : 8, LOSS>, 1024);
+        else go(teacher_row_kernel<TYPE, 1024, 0, LOSS>, 1024);
     });
     check_launch("teacher_row");
 }
