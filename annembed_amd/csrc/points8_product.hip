@@ -10,6 +10,8 @@
 // cores, and c of f32 takes the bf16 cores at half their rate: every value held is exact in bf16, the products too, the sums are f32.
 #include "points8.h"
 
+#include <algorithm>
+
 using namespace ae;
 
 namespace {
@@ -338,6 +340,102 @@ void product(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t c
     else launch_tiles<128, 128, 64>(x, p, dim, d_c, ctype, ldc, s);
 }
 
+// Up to 16 rows: bound by the points' bytes, which go from memory straight to the matrix cores (16 points a wave, 32 coordinates of a block
+// a lane).  Every workgroup quantises the rows itself, into LDS as the bf16 values they stand for, while its first points are on their way: one
+// launch.  SPLIT waves share the blocks of a group of points where there are few points.
+constexpr int kFew = 16;
+constexpr uint64_t few_lds_row(uint64_t dim) { return ((dim + kBlock - 1) / kBlock * kBlock) * 2 + 16; }   // (16 bytes more: neighbours start 4 banks apart)
+bool few_rows(uint64_t m, uint64_t dim) { return m <= kFew && m * few_lds_row(dim) <= 48 * 1024; }
+
+template <int XTYPE, int SPLIT>
+__global__ void __launch_bounds__(256) product_few_kernel(const typename Elem<XTYPE>::T* __restrict__ x, uint32_t m, uint64_t ldx, uint32_t dim, Rows8 p, void* c_, uint32_t ctype, uint64_t ldc) {
+    constexpr int GROUPS = 4 / SPLIT, AHEAD = 4;   // groups of 16 points a workgroup; blocks whose codes are fetched together
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
+    const uint32_t blocks = (dim + kBlock - 1) / kBlock, stride = (uint32_t)p.row_bytes, lds_row = blocks * (kBlock * 2) + 16;
+    const uint64_t j0 = (blockIdx.x * (uint64_t)GROUPS + wave / SPLIT) * 16;
+    const uint32_t nj = j0 < p.rows ? (uint32_t)min((uint64_t)16, p.rows - j0) : 0;
+    const uint64_t jb = nj ? j0 : 0;
+    __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc((void*)(p.codes + jb * stride), (short)0, (int)(nj * stride), 0x00027000);
+    const uint8_t* sp = p.scales + jb + (lane & 15);
+    const uint32_t row_at = (uint32_t)(lane & 15) * stride + g * 32;
+    u32x4 code[AHEAD][2];
+    uint32_t byte[AHEAD];
+    auto load = [&](uint32_t kb, int q) {   // (past the last block or a row's last byte: zeros)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t outside = kb * kBlock + g * 32 + h * 16 < stride ? 0u : 0x40000000u;
+            code[q][h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, (int)((row_at + kb * kBlock + h * 16) | outside), 0, 0));
+        }
+        byte[q] = sp[min(kb, blocks - 1) * p.scale_stride];
+    };
+    const uint32_t kb0 = SPLIT == 1 ? 0 : wave % SPLIT;
+#pragma unroll
+    for (int q = 0; q < AHEAD; q++) load(kb0 + q * SPLIT, q);
+    // the rows: as ae_points8_write holds them, 16 lanes a block
+    for (uint32_t u = tid >> 4; u < m * blocks; u += 16) {
+        const uint32_t i = u / blocks, b = u - i * blocks, k = b * kBlock + (lane & 15) * 8;
+        float v[8];
+        load8<XTYPE>(x + i * ldx + (k < dim ? k : 0), k < dim ? (int)min(8u, dim - k) : 0, v);
+        const uint32_t scale = scale_byte(max16(amax8(v)));
+        const uint2 e = encode8(v, scale);
+        *reinterpret_cast<bf16x8*>(lds + i * lds_row + k * 2) = widen8(e.x, e.y, scale);
+    }
+    __syncthreads();
+    const uint8_t* mine = lds + min((uint32_t)(lane & 15), m - 1) * lds_row + g * 64;   // (rows that do not exist repeat the last one, for nobody)
+    f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    for (uint32_t kb = kb0; kb < blocks; kb += AHEAD * SPLIT) {
+#pragma unroll
+        for (int q = 0; q < AHEAD; q++) {
+            const uint32_t at = min(kb + q * SPLIT, blocks - 1);   // (past the last block the codes are zeros)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const bf16x8 wp = widen8(code[q][e >> 1][(e & 1) * 2], code[q][e >> 1][(e & 1) * 2 + 1], byte[q]);
+                const bf16x8 wx = *reinterpret_cast<const bf16x8*>(mine + at * (kBlock * 2) + e * 16);
+                acc[e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp, wx, acc[e & 1], 0, 0, 0);
+            }
+            load(kb + (q + AHEAD) * SPLIT, q);
+        }
+    }
+    f32x4 sum = acc[0] + acc[1];
+    if constexpr (SPLIT > 1) {   // the waves' shares in order
+        __syncthreads();
+        f32x4* part = reinterpret_cast<f32x4*>(lds);
+        part[tid] = sum;
+        __syncthreads();
+        if (wave % SPLIT) return;
+#pragma unroll
+        for (int q = 1; q < SPLIT; q++) sum += part[tid + q * 64];
+    }
+    // a lane holds 4 consecutive points of row lane & 15
+    const uint32_t i = lane & 15;
+    if (i >= m) return;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t j = g * 4 + e;
+        if (j >= nj) continue;
+        const uint64_t at = i * ldc + j0 + j;
+        if (ctype == AE_TYPE_F32) static_cast<float*>(c_)[at] = sum[e];
+        else if (ctype == AE_TYPE_BF16) static_cast<__bf16*>(c_)[at] = (__bf16)sum[e];
+        else static_cast<_Float16*>(c_)[at] = (_Float16)sum[e];
+    }
+}
+
+void product_few(const void* d_x, uint32_t xtype, uint64_t m, uint64_t ldx, uint64_t dim, const Rows8& p, void* d_c, uint32_t ctype, uint64_t ldc, hipStream_t s) {
+    const unsigned bytes = (unsigned)std::max<uint64_t>(m * few_lds_row(dim), 4096);
+    by_type(xtype, [&](auto ty) {
+        constexpr int TYPE = decltype(ty)::value;
+        auto go = [&](auto kernel, unsigned points) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((p.rows + points - 1) / points)), dim3(256), bytes, s, static_cast<const typename Elem<TYPE>::T*>(d_x), (uint32_t)m, ldx,
+                               (uint32_t)dim, p, d_c, ctype, ldc);
+        };
+        // 16 points a wave leave half of the chip's waves without work below 32 768 points: four waves share them then
+        if (p.rows >= 32768 || points8_blocks(dim) < 4) go(product_few_kernel<TYPE, 1>, 64);
+        else go(product_few_kernel<TYPE, 4>, 16);
+    });
+    check_launch("points8_product_few");
+}
+
 uint64_t product_work(uint64_t m, uint64_t dim) { return m * points8_row_bytes(dim) + points8_blocks(dim) * points8_scale_stride(m) + kScaleSlack; }
 
 }  // namespace
@@ -348,7 +446,7 @@ int32_t ae_points8_product_work(const ae_points8* p, uint64_t n, uint64_t m, uin
     return guard([&] {
         if (!p || !bytes) fail(AE_ERR_INVALID_ARG, "ae_points8_product_work: null argument");
         if (m > (1ull << 32)) fail(AE_ERR_INVALID_ARG, "ae_points8_product_work: %llu rows are out of range", (unsigned long long)m);
-        *bytes = product_work(m, p->dim);
+        *bytes = m && n && !few_rows(m, p->dim) ? product_work(m, p->dim) : 0;
     });
 }
 
@@ -362,6 +460,7 @@ int32_t ae_points8_product(const ae_points8* p, uint64_t first, uint64_t n, cons
         if (n == 0 || m == 0) return;
         check_rows(d_x, xtype, m, p->dim, ldx, "ae_points8_product: x");
         check_rows(d_c, ctype, m, n, ldc, "ae_points8_product: c");
+        if (few_rows(m, p->dim)) return product_few(d_x, xtype, m, ldx, p->dim, points8_rows(p, first, n), d_c, ctype, ldc, (hipStream_t)stream);
         const uint64_t need = product_work(m, p->dim);
         if (!d_work || work_bytes < need) fail(AE_ERR_INVALID_ARG, "ae_points8_product: %llu bytes of scratch are needed, %llu given", (unsigned long long)need, (unsigned long long)work_bytes);
         check_aligned(d_work, 16, "ae_points8_product: work");
