@@ -47,10 +47,11 @@ __global__ void __launch_bounds__(256) points8_release_kernel(const uint32_t* __
     if (s < capacity) owner[s] = 0;
 }
 
-// SLOTS 0: row i to first + i.  1: to slots[i], each row scans for a later row of the same slot.  2: to slots[i] where owner says so.
+// SLOTS 0: row i to first + i.  1: to slots[i], each row scans for a later row of the same slot.  2: to slots[i] where owner says so.  3: the same
+// for rows of one block, which give their slot back themselves (another row of that slot finds the owner or nobody: not itself).
 template <int TYPE, int SLOTS>
 __global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<TYPE>::T* __restrict__ x, uint64_t ldx, uint64_t dim, Blocks bl, uint64_t first,
-                                                            const uint32_t* __restrict__ slots, const uint32_t* __restrict__ owner, uint64_t capacity,
+                                                            const uint32_t* __restrict__ slots, uint32_t* __restrict__ owner, uint64_t capacity,
                                                             uint8_t* __restrict__ codes, uint64_t row_bytes, uint8_t* __restrict__ scales, uint64_t scale_stride) {
     const uint64_t u0 = blockIdx.x * (uint64_t)(kGroups * kTrips);
     const Cursor cur(u0, bl.nb);
@@ -77,7 +78,8 @@ __global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<
                 const uint32_t s = slots[row[t]];
                 to = s;
                 live[t] = s < capacity;
-                if constexpr (SLOTS == 2) live[t] = live[t] && owner[s] == (uint32_t)row[t] + 1;
+                if constexpr (SLOTS >= 2) live[t] = live[t] && owner[s] == (uint32_t)row[t] + 1;
+                if constexpr (SLOTS == 3) { if (live[t] && lane == 0) owner[s] = 0; }
             }
             if constexpr (SLOTS == 1) {
                 bool later = false;
@@ -154,7 +156,7 @@ unsigned trips_grid(const Blocks& bl) {
 }
 
 template <int SLOTS>
-void launch_write(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint64_t first, const uint32_t* slots, const uint32_t* owner, uint64_t capacity,
+void launch_write(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint64_t first, const uint32_t* slots, uint32_t* owner, uint64_t capacity,
                   uint8_t* codes, uint8_t* scales, uint64_t scale_stride, hipStream_t s) {
     const Blocks bl = blocks_of(n, dim);
     const unsigned grid = trips_grid(bl);
@@ -262,7 +264,7 @@ int32_t ae_points8_write(ae_points8* p, const void* d_x, uint32_t type, uint64_t
         check_aligned(d_slots, 4, "ae_points8_write: slots");
         if (n > 0x7FFFFFFFull) fail(AE_ERR_INVALID_ARG, "ae_points8_write: %llu slots are more than one call takes", (unsigned long long)n);
         // The last row of a repeated slot is held.  Few rows: every block scans the slots behind its own, one launch.  More: the rows claim
-        // their slots first and give them back afterwards, three launches.
+        // their slots first and give them back as they are written, or, rows of several blocks, in a launch of their own.
         if (n <= kScan) {
             launch_write<1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
             return;
@@ -270,6 +272,10 @@ int32_t ae_points8_write(ae_points8* p, const void* d_x, uint32_t type, uint64_t
         const unsigned grid = blocks_for(n, 256);
         hipLaunchKernelGGL(points8_claim_kernel, dim3(grid), dim3(256), 0, s, d_slots, (uint32_t)n, p->capacity, p->owner.p);
         check_launch("points8_claim");
+        if (p->blocks == 1) {
+            launch_write<3>(d_x, type, n, ldx, p->dim, 0, d_slots, p->owner.p, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
+            return;
+        }
         launch_write<2>(d_x, type, n, ldx, p->dim, 0, d_slots, p->owner.p, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
         hipLaunchKernelGGL(points8_release_kernel, dim3(grid), dim3(256), 0, s, d_slots, (uint32_t)n, p->capacity, p->owner.p);
         check_launch("points8_release");

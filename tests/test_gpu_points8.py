@@ -76,11 +76,11 @@ def test_special_values(A):
     np.testing.assert_array_equal(n64(bank.read()), U.values(x))
 
 
-@pytest.mark.parametrize("n", [5, 1024, 1025, 5000])
-def test_slots(A, n):
-    """scattered, padded, repeated and invalid slots, on both sides of the size where the rows claim their slots; twice in a row"""
+@pytest.mark.parametrize("n,dim", [(5, 200), (1024, 200), (1025, 200), (5000, 200), (1025, 128), (5000, 28)])
+def test_slots(A, n, dim):
+    """scattered, padded, repeated and invalid slots, on both sides of the size where the rows claim their slots, of one block and more; twice"""
     rng = np.random.default_rng(n)
-    cap, dim = 3000, 200
+    cap = 3000
     bank = A.Points8(cap, dim)
     held = np.zeros((cap, dim))
     for turn in range(2):
