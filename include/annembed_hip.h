@@ -660,7 +660,7 @@ enum { AE_TEACHER_PROBA = 0, AE_TEACHER_LOGITS = 1 };
 int32_t ae_teacher_loss(const void *d_logits, uint32_t type, uint64_t rows, uint64_t cols, uint64_t ld, const uint32_t *d_idx,
                         const float *d_list, uint32_t k, uint64_t ldk, uint32_t kind, float temperature, const float *d_row_weight,
                         float *d_loss, float *d_stats, void *d_grad, uint64_t ldg, void *d_work, uint64_t work_bytes, void *stream);
-int32_t ae_teacher_loss_work(uint64_t rows, uint64_t cols, uint64_t *bytes);
+int32_t ae_teacher_loss_work(uint64_t rows, uint64_t cols, uint64_t *bytes); /* whatever the type, with or without the gradient */
 /* The gradient from the statistics of an earlier ae_teacher_loss on the same logits, under each row's own upstream gradient: w_r above is
    d_dloss[r] (include the row's weight in it).  d_grad may be d_logits. */
 int32_t ae_teacher_grad(const void *d_logits, uint32_t type, uint64_t rows, uint64_t cols, uint64_t ld, const float *d_stats,
