@@ -321,7 +321,10 @@ int32_t ae_points8_product_grad(const ae_points8* p, uint64_t first, uint64_t n,
         if (g.bytes && (!d_work || work_bytes < g.bytes))
             fail(AE_ERR_INVALID_ARG, "ae_points8_product_grad: %llu bytes of scratch are needed, %llu given", (unsigned long long)g.bytes, (unsigned long long)work_bytes);
         check_aligned(d_work, 16, "ae_points8_product_grad: work");
-        if (g.tiles_m * g.tiles_k * g.slices > 0x3FFFFFull) fail(AE_ERR_INVALID_ARG, "ae_points8_product_grad: %llu rows are more than one call takes", (unsigned long long)m);
+        const unsigned groups = g.slices >= 64 ? 16 : g.slices >= 8 ? 4 : 1;   // (the join's)
+        const uint64_t runs = m * (g.ldp / 4);
+        if (g.tiles_m * g.tiles_k * g.slices > 0x3FFFFFull || runs * groups > 0xFFFF0000ull)
+            fail(AE_ERR_INVALID_ARG, "ae_points8_product_grad: %llu rows are more than one call takes", (unsigned long long)m);
         if (n) {
             const uint64_t tiles = g.tiles_m * g.tiles_k;
             GradArgs a{d_dc, lddc, m, n, p->dim, points8_rows(p, first, n), g.per_slice, (float*)d_work, g.ldp, (uint32_t)g.tiles_k, (uint32_t)tiles, (uint32_t)g.slices};
@@ -339,14 +342,13 @@ int32_t ae_points8_product_grad(const ae_points8* p, uint64_t first, uint64_t n,
         }
         by_type(xtype, [&](auto ty) {
             constexpr int TYPE = decltype(ty)::value;
-            const uint64_t runs = m * (g.ldp / 4);
-            auto go = [&](auto kernel, unsigned groups) {
+            auto go = [&](auto kernel) {
                 hipLaunchKernelGGL(kernel, dim3(blocks_for(runs * groups, 256)), dim3(256), 0, s, (const float*)d_work, (uint32_t)g.slices, m, p->dim, g.ldp,
                                    static_cast<typename Elem<TYPE>::T*>(d_dx), lddx);
             };
-            if (g.slices >= 64) go(grad_join_kernel<TYPE, 16>, 16);
-            else if (g.slices >= 8) go(grad_join_kernel<TYPE, 4>, 4);
-            else go(grad_join_kernel<TYPE, 1>, 1);
+            if (groups == 16) go(grad_join_kernel<TYPE, 16>);
+            else if (groups == 4) go(grad_join_kernel<TYPE, 4>);
+            else go(grad_join_kernel<TYPE, 1>);
         });
         check_launch("points8_grad_join");
     });

@@ -345,7 +345,7 @@ void product(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t c
 // launch.  SPLIT waves share the blocks of a group of points where there are few points.
 constexpr int kFew = 16;
 constexpr uint64_t few_lds_row(uint64_t dim) { return ((dim + kBlock - 1) / kBlock * kBlock) * 2 + 16; }   // (16 bytes more: neighbours start 4 banks apart)
-bool few_rows(uint64_t m, uint64_t dim) { return m <= kFew && m * few_lds_row(dim) <= 48 * 1024; }
+bool few_rows(uint64_t m, uint64_t n, uint64_t dim) { return m <= kFew && m * few_lds_row(dim) <= 48 * 1024 && n < 1ull << 30; }   // (64 points, 256 threads: below 2^32)
 
 template <int XTYPE, int SPLIT>
 __global__ void __launch_bounds__(256) product_few_kernel(const typename Elem<XTYPE>::T* __restrict__ x, uint32_t m, uint64_t ldx, uint32_t dim, Rows8 p, void* c_, uint32_t ctype, uint64_t ldc) {
@@ -446,7 +446,7 @@ int32_t ae_points8_product_work(const ae_points8* p, uint64_t n, uint64_t m, uin
     return guard([&] {
         if (!p || !bytes) fail(AE_ERR_INVALID_ARG, "ae_points8_product_work: null argument");
         if (m > (1ull << 32)) fail(AE_ERR_INVALID_ARG, "ae_points8_product_work: %llu rows are out of range", (unsigned long long)m);
-        *bytes = m && n && !few_rows(m, p->dim) ? product_work(m, p->dim) : 0;
+        *bytes = m && n && !few_rows(m, n, p->dim) ? product_work(m, p->dim) : 0;
     });
 }
 
@@ -460,7 +460,7 @@ int32_t ae_points8_product(const ae_points8* p, uint64_t first, uint64_t n, cons
         if (n == 0 || m == 0) return;
         check_rows(d_x, xtype, m, p->dim, ldx, "ae_points8_product: x");
         check_rows(d_c, ctype, m, n, ldc, "ae_points8_product: c");
-        if (few_rows(m, p->dim)) return product_few(d_x, xtype, m, ldx, p->dim, points8_rows(p, first, n), d_c, ctype, ldc, (hipStream_t)stream);
+        if (few_rows(m, n, p->dim)) return product_few(d_x, xtype, m, ldx, p->dim, points8_rows(p, first, n), d_c, ctype, ldc, (hipStream_t)stream);
         const uint64_t need = product_work(m, p->dim);
         if (!d_work || work_bytes < need) fail(AE_ERR_INVALID_ARG, "ae_points8_product: %llu bytes of scratch are needed, %llu given", (unsigned long long)need, (unsigned long long)work_bytes);
         check_aligned(d_work, 16, "ae_points8_product: work");

@@ -4,6 +4,8 @@
 // g P q_v everywhere and g (P q_v - p) at the k listed columns.  Two floating point operations and an exponential per logit: bound by HBM.
 #include "points8.h"
 
+#include <cfloat>
+
 using namespace ae;
 
 namespace {
@@ -396,7 +398,8 @@ __global__ void __launch_bounds__(kSliceThreads) teacher_slope_kernel(const type
 
 void check_size(uint64_t rows, uint64_t cols, const char* what) {
     if (cols == 0 || cols >= 0xFFFFFFFFull) fail(AE_ERR_INVALID_ARG, "%s: %llu columns are out of range", what, (unsigned long long)cols);
-    if (rows > 0xFFFFFFull || rows * ((cols + kHeld - 1) / kHeld) > 0xFFFFFFull)
+    const uint64_t threads = cols <= 8192 ? 256 : (cols + 8191) / 8192 * 512;   // the most that a row gets; a launch has fewer than 2^32
+    if (rows > 0xFFFFFFull || rows * threads > 0xFFFFFFFFull)
         fail(AE_ERR_INVALID_ARG, "%s: %llu rows of %llu columns are more than one call takes", what, (unsigned long long)rows, (unsigned long long)cols);
 }
 void check_list(const uint32_t* d_idx, const float* d_list, uint32_t k, uint64_t ldk, uint32_t kind, float temperature, uint64_t rows, uint64_t cols, const char* what) {
@@ -404,7 +407,8 @@ void check_list(const uint32_t* d_idx, const float* d_list, uint32_t k, uint64_t
     if (k == 0 || k > kMaxList) fail(AE_ERR_INVALID_ARG, "%s: a list of %u entries is not in [1, %u]", what, k, kMaxList);
     if (ldk < k) fail(AE_ERR_INVALID_ARG, "%s: the list's stride is shorter than the list", what);
     if (kind > AE_TEACHER_LOGITS) fail(AE_ERR_INVALID_ARG, "%s: unknown kind of list %u", what, kind);
-    if (!(temperature > 0.f) || !(temperature < INFINITY)) fail(AE_ERR_INVALID_ARG, "%s: the temperature has to be positive", what);
+    if (ldk > (1ull << 40) / rows) fail(AE_ERR_INVALID_ARG, "%s: %llu lists of stride %llu are out of range", what, (unsigned long long)rows, (unsigned long long)ldk);
+    if (!(temperature >= FLT_MIN) || !(temperature < INFINITY)) fail(AE_ERR_INVALID_ARG, "%s: the temperature has to be positive, finite and not denormal", what);
     check_size(rows, cols, what);
     check_aligned(d_idx, 4, what);
     check_aligned(d_list, 4, what);

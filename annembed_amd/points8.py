@@ -155,9 +155,10 @@ class Points8:
     def read(self, n=None, first=0, slots=None, dtype=torch.float32, out=None):
         """the values held in points first ... first + n - 1, or in `slots` (-1 reads as zeros, others outside the store as NaN)"""
         if slots is not None:
-            if n is not None and n != slots.shape[0]:
-                raise _bad("%s points from %d slots" % (n, slots.shape[0]))
-            n, first = slots.shape[0], 0
+            many = slots.numel() if isinstance(slots, torch.Tensor) else 0
+            if n is not None and n != many:
+                raise _bad("%s points from %d slots" % (n, many))
+            n, first = many, 0
         else:
             n, first = self._range(n, first)
         s = _vector(slots, "slots", self.device, n, _INDEX)

@@ -597,7 +597,8 @@ int32_t ae_embedder_get_quality_estimate_from_edge_length(const ae_embedder *e, 
  * calls, so they may be captured into a graph.  Scratch memory is the caller's: the *_work functions say how many bytes a call of
  * that size needs (0: d_work may be NULL); it has to be 16-byte aligned and two calls that may run at the same time need scratch of their own.
  * Rows are row-major with a stride of ld* ELEMENTS (>= the row's length; rows of an even 16 bytes are read fastest, any alignment of an
- * element's size works).  n, m, rows = 0 is a call that does nothing.
+ * element's size works).  n, m, rows = 0 is a call that does nothing.  What a call writes overlaps nothing that it reads, but where it says so.
+ * Sizes that need 2^32 threads or more in one launch are refused.
  *
  * Format: a row of `dim` coordinates in blocks of 128 (the last may be shorter).  a = the largest magnitude among the finite values of the
  * block, e = the smallest integer >= -126 with a <= 448 * 2^e.  A coordinate is the e4m3 number nearest to x * 2^-e (ties to even); NaN
@@ -650,7 +651,7 @@ int32_t ae_kgraph_bruteforce_l2_points8(const ae_points8 *p, uint64_t first, uin
      AE_TEACHER_LOGITS  the teacher's logit t_j: p = softmax(t / temperature) over the row's list (-inf: p = 0).
    With ln q = ln softmax(s / temperature):   loss_r = w_r sum_j p_j (ln p_j - ln q_{idx_j}),   w_r = d_row_weight[r] (NULL: 1)
                                                d loss_r / d s_v = w_r (q_v sum_j p_j - sum_{j: idx_j = v} p_j) / temperature.
-   A column may come several times in a list: its probabilities add up.  p_j = 0 contributes nothing; p_j > 0 on a logit of -inf makes the
+   The temperature is positive, finite and not denormal.  A column may come several times in a list: its probabilities add up.  p_j = 0 contributes nothing; p_j > 0 on a logit of -inf makes the
    loss +inf.  A row of weight 0 is not looked at (its logits and list may hold anything): loss 0, gradient 0; so are rows whose logits
    are all -inf.  A column index >= cols, a NaN or a +inf among a row's logits makes that row NaN.
    d_loss[rows] f32; d_stats[rows][2] f32: (the largest logit, ln sum_v exp((s_v - largest) / temperature)), (-inf, 0) for rows left out --

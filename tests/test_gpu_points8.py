@@ -333,3 +333,85 @@ def test_refusals(A):
     assert lib.ae_points8_product(bank.handle, 0, 100, many.data_ptr(), 0, 30, 64, c.data_ptr(), 0, 100, None, 0, None) == L.AE_ERR_INVALID_ARG
     assert b"scratch" in lib.ae_last_error_message()
     assert lib.ae_points8_read(bank.handle, 0, None, 0, None, 0, 0, None) == L.AE_OK
+
+
+def test_strides_of_gigabytes(A):
+    """rows of dc, of dx and of the product so far apart that a tile of them spans more than 32-bit offsets reach; few and more rows"""
+    n, dim = 300, 130
+    bank = A.Points8(n, dim)
+    p = vectors(n, dim, 1)
+    bank.write(p.cuda())
+    pv = U.values(n64(p))
+    step = 9_000_000
+    for m in (3, 20):
+        room = torch.zeros((m - 1) * step + n, dtype=torch.bfloat16, device="cuda")
+        dc = vectors(m, n, 2).bfloat16()
+        far = room.as_strided((m, n), (step, 1))
+        far.copy_(dc)
+        got, want = n64(bank.product_grad(far)), n64(dc) @ pv
+        assert (np.abs(got - want) <= product_bound(n64(dc), pv, 3 * n + 64, want, torch.float32)).all()
+        x = vectors(m, dim, 3)
+        xv = U.values(n64(x))
+        bank.product(x.cuda(), out=far)
+        assert (np.abs(n64(far) - xv @ pv.T) <= product_bound(xv, pv.T, dim, xv @ pv.T, torch.bfloat16, eights=True)).all()
+        assert not room.as_strided((m - 1, step - n), (step, 1), n).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradient_that_ends_with_a_page(A, dtype):
+    """an odd number of 16-bit values whose last one is the last of a page: the copies may not take the dword that it starts"""
+    n, dim, m = 129, 40, 5
+    bank = A.Points8(n, dim)
+    p = vectors(n, dim, 1)
+    bank.write(p.cuda())
+    pv = U.values(n64(p))
+    room = torch.full((8192,), float("nan"), dtype=dtype, device="cuda")
+    end = 2048 * 3 - room.data_ptr() % 4096 // 2   # elements to a page's end
+    dc = vectors(m, n, 2).to(dtype)
+    for last in (end, end - 1):   # (the other one may, and what it takes there is NaN)
+        view = room[last - m * n:last].view(m, n)
+        view.copy_(dc)
+        assert (view.data_ptr() + 2 * m * n) % 4096 == (0 if last == end else 4094)
+        got, want = n64(bank.product_grad(view)), n64(dc) @ pv
+        assert (np.abs(got - want) <= product_bound(n64(dc), pv, 3 * n + 64, want, torch.float32)).all()
+        room.fill_(float("nan"))
+
+
+def test_the_same_store_on_both_sides_and_views_of_it(A):
+    """products of a store with itself, a part with another; the store's memory outlives the object that views of it came from"""
+    x = vectors(200, 96, 1)
+    bank = A.Points8(200, 96)
+    bank.write(x.cuda())
+    v = U.values(n64(x))
+    got = n64(bank.product(bank, n=50, first=150, x_first=7, m=120))
+    want = v[7:127] @ v[150:].T
+    assert (np.abs(got - want) <= product_bound(v[7:127], v[150:].T, 96, want, torch.float32)).all()
+    codes, scales = bank.codes(), bank.scales()
+    keep = codes.float() * torch.exp2(scales.float() - 127)
+    del bank
+    other = A.Points8(200, 96)
+    other.write(torch.ones(200, 96, device="cuda"))
+    assert torch.equal(codes.float() * torch.exp2(scales.float() - 127), keep)
+
+
+def test_rows_behind_the_last_point_do_not_count(A):
+    """points behind the range that is asked for hold NaN, so do the rows' neighbours in memory"""
+    bank = A.Points8(64, 100)
+    bank.write(torch.full((64, 100), float("nan"), device="cuda"))
+    p = vectors(20, 100, 1)
+    bank.write(p.cuda(), first=16)
+    pv = U.values(n64(p))
+    for m in (2, 30):
+        room = torch.full((m + 2, 120), float("nan"), device="cuda")
+        x = vectors(m, 100, 2)
+        room[1:-1, 8:108] = x.cuda()
+        xv = U.values(n64(x))
+        for dtype in TYPES:
+            got = n64(bank.product(room[1:-1, 8:108], n=20, first=16, dtype=dtype))
+            fits = np.abs(xv @ pv.T) < (65000 if dtype == torch.float16 else np.inf)   # (beyond, f16 has its infinities)
+            assert (np.abs(got - xv @ pv.T) <= product_bound(xv, pv.T, 100, xv @ pv.T, dtype, eights=dtype != torch.float32))[fits].all()
+            wide = torch.full((m + 2, 33), float("nan"), dtype=dtype, device="cuda")
+            dc = vectors(m, 20, 3).to(dtype)
+            wide[1:-1, 5:25] = dc.cuda()
+            got, want = n64(bank.product_grad(wide[1:-1, 5:25], n=20, first=16)), n64(dc) @ pv
+            assert (np.abs(got - want) <= product_bound(n64(dc), pv, 3 * 20 + 64, want, torch.float32)).all()
