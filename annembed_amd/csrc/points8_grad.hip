@@ -4,11 +4,8 @@
 // run of the summed axis.  But code * 2^e is exact in bf16, and dc of f32 (f16) is the sum of three (two) bf16 numbers, so bf16 matrix cores
 // compute the product of the values themselves with f32 sums: nothing is rounded before the result.
 //
-// A workgroup owns 64 FR rows x 128 coordinates (one block: one scale byte per point) and walks a slice of the points 64 at a time; a wave owns
-// 16 FR of the rows and all coordinates.  dc goes to LDS as it is, three steps deep.  (Straight to the lanes that multiply it, 16 bytes of 16
-// rows each, every lane would be an access of its own to the cache: 57 us where this takes 4x fewer.)  The codes are turned on the way to LDS:
-// a thread takes 4 coordinates of 8 points, widens them under the products of the step before and writes 8 points of one coordinate as 16
-// bytes.  One barrier a step.  Few rows leave few tiles: the points are split into slices whose sums are joined in order.
+// A workgroup owns 64 or 128 rows x 128 coordinates (one block: one scale byte per point) and walks a slice of the points 64 at a time.  Few rows leave
+// few tiles: the points are split into slices whose sums are joined in order; one slice writes the result itself.
 #include "points8.h"
 
 using namespace ae;
@@ -16,6 +13,7 @@ using namespace ae;
 namespace {
 
 constexpr int kStep = 64;    // points per step: 128 bytes of bf16
+constexpr uint32_t kPast = 0x3FFF0000u;      // the ranges of a tile's rows of dc and of a slice's codes do not reach this far
 constexpr uint32_t kOutside = 0x40000000u;   // an offset outside every buffer's range (dc's rows of a tile, a slice's codes: less than 1 GiB)
 
 template <int TYPE> constexpr int terms_of() { return TYPE == AE_TYPE_F32 ? 3 : TYPE == AE_TYPE_F16 ? 2 : 1; }
@@ -28,23 +26,30 @@ __device__ __forceinline__ int at_coords(int k, int chunk) { return k * 128 + ((
 // a row of dc: 8 (f32: 16) pieces of 16 bytes
 template <int PIECES> __device__ __forceinline__ int turn(int r) { return PIECES == 8 ? (r >> 1) & 7 : r & 15; }
 
-// eight values as the sum of TERMS bf16 numbers, the first ones cut off (never past the largest bf16): exact apart from what lies below bf16's range
+// Eight values as the sum of TERMS bf16 numbers, each the upper half of what the ones before it leave: exact (8 + 8 + 8 bits of f32's 24, 8 + 8 of f16's
+// 11) apart from what lies below bf16's range.  An infinity leaves nothing; what a NaN leaves is NaN, whatever its upper half says.
 template <int TYPE>
 __device__ __forceinline__ void split8(const typename Elem<TYPE>::T (&v)[8], bf16x8 (&t)[terms_of<TYPE>()]) {
     constexpr int TERMS = terms_of<TYPE>();
+    if constexpr (TERMS == 1) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        if constexpr (TERMS == 1) t[0][e] = (__bf16)v[e];
-        else {
-            float r = (float)v[e];
-            const bool finite = (__float_as_uint(r) & 0x7FFFFFFFu) < 0x7F800000u;
+        for (int e = 0; e < 8; e++) t[0][e] = (__bf16)v[e];
+    } else {
+        uint32_t r[8];
 #pragma unroll
-            for (int q = 0; q + 1 < TERMS; q++) {
-                const float cut = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u);
-                t[q][e] = finite ? (__bf16)cut : (__bf16)r;
-                r = finite ? r - cut : 0.f;
+        for (int e = 0; e < 8; e++) r[e] = __float_as_uint((float)v[e]);
+#pragma unroll
+        for (int q = 0; q < TERMS; q++) {
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(r[2 * e + 1], r[2 * e], 0x07060302u);
+            t[q] = __builtin_bit_cast(bf16x8, w);
+            if (q + 1 == TERMS) break;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float x = __uint_as_float(r[e]), left = x - __uint_as_float(r[e] & 0xFFFF0000u);
+                r[e] = __float_as_uint(q == 0 && __builtin_amdgcn_classf(x, 0x204) ? 0.f : left);   // (0x204: the infinities)
             }
-            t[TERMS - 1][e] = (__bf16)r;
         }
     }
 }
@@ -58,8 +63,45 @@ struct GradArgs {
     float* part;          // [slices][m][ldp]
     uint64_t ldp;
     uint32_t tiles_k, tiles, slices;
+    void* dx;             // one slice: its sums are the result, rounded here
+    uint32_t xtype;
+    uint64_t lddx;
 };
 
+// sums of 4 coordinates from k on, of row r
+__device__ __forceinline__ void put(const GradArgs& a, uint32_t slice, uint64_t r, uint64_t k, f32x4 v) {
+    if (a.slices > 1) {
+        if (k < a.ldp) *reinterpret_cast<f32x4*>(a.part + (slice * a.m + r) * a.ldp + k) = v;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (k + e >= a.dim) return;
+        const uint64_t at = r * a.lddx + k + e;
+        if (a.xtype == AE_TYPE_F32) static_cast<float*>(a.dx)[at] = v[e];
+        else if (a.xtype == AE_TYPE_BF16) static_cast<__bf16*>(a.dx)[at] = (__bf16)v[e];
+        else static_cast<_Float16*>(a.dx)[at] = (_Float16)v[e];
+    }
+}
+
+// The slice and tile of a workgroup.  Workgroups go to the 8 XCDs in turn, each with an L2 of its own: an XCD owns a run of slices, all tiles of
+// a slice one after the other, so that dc and the points are fetched from memory once and shared there.
+__device__ __forceinline__ bool place_of(const GradArgs& a, uint32_t& slice, uint32_t& ti, uint32_t& tk) {
+    const uint32_t total = a.tiles * a.slices, each = total / 8, more = total % 8, xcd = blockIdx.x % 8, at = blockIdx.x / 8;
+    if (at >= each + (xcd < more ? 1 : 0)) return false;
+    const uint32_t id = xcd * each + min(xcd, more) + at;
+    slice = __builtin_amdgcn_readfirstlane(id / a.tiles);
+    const uint32_t tile = id - slice * a.tiles;
+    ti = __builtin_amdgcn_readfirstlane(tile / a.tiles_k);
+    tk = tile - ti * a.tiles_k;
+    return true;
+}
+
+// dc of f32 and f16 (and of any type whose rows lie too far apart for 32-bit offsets, or that ends in half a dword with its page).  A wave owns 16 FR of
+// the rows and all coordinates, so each value of dc is split once.  dc goes to LDS as it is, three steps deep.  (Straight to the lanes that
+// multiply it, 16 bytes of 16 rows each, every lane would be an access of its own to the cache.)  The codes are turned on the way to LDS: a thread takes
+// 4 coordinates of 8 points, widens them under the products of the step before and writes 8 points of one coordinate as 16 bytes.  One
+// barrier a step.  8192 x 8192 x 4096 of f32: 970 TF of the three partial products, at the rate of the matrix cores; 300 x 60 000 x 784: 107 us.
 template <int TYPE, int FR> constexpr int grad_lds() { return 3 * 64 * FR * kStep * (TYPE == AE_TYPE_F32 ? 4 : 2) + 2 * kBlock * 128; }   // 56 or 80 KB: two workgroups a CU
 
 template <int TYPE, int FR, bool VEC>   // VEC: the copies' 32-bit offsets and whole pieces do for dc
@@ -67,11 +109,8 @@ __global__ void __launch_bounds__(256, 2) grad_tile_kernel(GradArgs a) {
     using T = typename Elem<TYPE>::T;
     constexpr int TERMS = terms_of<TYPE>(), ROW = kStep * (int)sizeof(T), PIECES = ROW / 16, STAGE = 64 * FR * ROW, COPIES = STAGE / 4096;
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];   // three stages of dc, two of coordinates
-    // Workgroups go to the 8 XCDs in turn, each with an L2 of its own: an XCD owns a run of slices, all tiles of a slice one after the other, so
-    // that dc and the points are fetched from memory once and shared there.
-    const uint32_t total = a.tiles * a.slices, each = total / 8, more = total % 8, xcd = blockIdx.x % 8, at = blockIdx.x / 8;
-    if (at >= each + (xcd < more ? 1 : 0)) return;
-    const uint32_t id = xcd * each + min(xcd, more) + at, slice = id / a.tiles, tile = id - slice * a.tiles, ti = tile / a.tiles_k, tk = tile - ti * a.tiles_k;
+    uint32_t slice, ti, tk;
+    if (!place_of(a, slice, ti, tk)) return;
     const uint64_t i0 = (uint64_t)ti * (64 * FR), k0 = (uint64_t)tk * kBlock;
     const uint64_t jb = slice * a.per_slice, je = min(a.n, jb + a.per_slice);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
@@ -220,17 +259,187 @@ __global__ void __launch_bounds__(256, 2) grad_tile_kernel(GradArgs a) {
     } else step(t, even, std::true_type{});
     if constexpr (VEC) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the copies for nobody have ended before the LDS is given back
     // coordinates are the matrix cores' rows: a lane holds runs of 4 consecutive k of its rows
-    float* part = a.part + slice * (a.m * a.ldp);
 #pragma unroll
     for (int i = 0; i < FR; i++) {
         const uint64_t r = i0 + r0 + i * 16;
         if (r >= a.m) continue;
 #pragma unroll
-        for (int q = 0; q < 8; q++) {
-            const uint64_t k = k0 + q * 16 + g * 4;
-            if (k < a.ldp) *reinterpret_cast<f32x4*>(part + r * a.ldp + k) = acc[i][q];
-        }
+        for (int q = 0; q < 8; q++) put(a, slice, r, k0 + q * 16 + g * 4, acc[i][q]);
     }
+}
+
+// dc of bf16, which the matrix cores take as it is.  16 FR rows x 128 coordinates; two waves share the coordinates, two the points of a step.  A lane
+// takes 4 coordinates of 8 points, one dword a point: put together by coordinate they are what the matrix cores want of it, with coordinates 4 apart
+// in a fragment, so the codes are widened in the registers they are used from, and each wave reads all rows of dc: LDS moves 48 KB for
+// 128 x 128 x 64 where the kernel above moves 112 (300 x 60 000 x 784: 49 us against 52, 4096 x 32 768 x 1024: 256 against 303, 1075 TF of the 1413 that a
+// large bf16 product of the library reaches).  dc and the codes come by copies to LDS three deep; the codes are read two steps ahead and widened under
+// the products, whose waits for one another and for the barrier of a step are what bounds it: the matrix cores are busy for 45 % of the time.
+constexpr int kTurnStage = kStep * 128;   // codes of a step
+template <int FR> constexpr int turn_lds() { return 3 * (16 * FR * kStep * 2 + kTurnStage + 1024); }   // 51 or 75 KB for 64 or 128 rows
+
+template <int FR>
+__global__ void __launch_bounds__(256, FR == 8 ? 2 : FR == 4 ? 3 : 4) grad_turn_kernel(GradArgs a) {
+    constexpr int STAGE = 16 * FR * kStep * 2, CODES = 3 * STAGE, SCALES = CODES + 3 * kTurnStage, COPIES_DC = FR / 2, COPIES = COPIES_DC + 3;
+    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
+    uint32_t slice, ti, tk;
+    if (!place_of(a, slice, ti, tk)) return;
+    const uint64_t i0 = (uint64_t)ti * (16 * FR), k0 = (uint64_t)tk * kBlock;
+    const uint64_t jb = slice * a.per_slice, je = min(a.n, jb + a.per_slice);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
+    const int half = wave >> 1, side = wave & 1, mine = part(half, g);   // of the points, of the coordinates; this lane's 8 points of the step's 64
+    const uint32_t mi = (uint32_t)min((uint64_t)(16 * FR), a.m - i0), points = (uint32_t)(je - jb), steps = (points + kStep - 1) / kStep;
+    const __bf16* dc = static_cast<const __bf16*>(a.dc) + i0 * a.lddc + jb;
+    // ---- the copies.  Ranges and what lies behind the last point: as above
+    const uint32_t row_bytes = (uint32_t)a.lddc * 2, stride = (uint32_t)a.p.row_bytes;
+    __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)dc, (short)0, (int)((mi - 1) * row_bytes + (points * 2 + 3) / 4 * 4), 0x00027000);
+    __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.codes + jb * stride), (short)0, (int)(points * stride), 0x00027000);
+    __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.scales + tk * a.p.scale_stride + jb), (short)0, (int)(points + 256), 0x00027000);   // (kScaleSlack)
+    const int copy_row = wave * 8 + (lane >> 3), copy_piece = (lane & 7) ^ turn<8>(copy_row);
+    const uint32_t dc_at = copy_row * row_bytes + copy_piece * 16;
+    auto copy_dc = [&](uint32_t step, uint32_t stage) {   // (zeros for a step that does not exist)
+#pragma unroll
+        for (int q = 0; q < COPIES_DC; q++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rd, (__attribute__((address_space(3))) void*)(lds + stage * STAGE + (q * 4 + wave) * 1024), 16,
+                                                     (int)dc_at, (int)(step < steps ? step * (kStep * 2) + q * 32 * row_bytes : kPast), 0, 0);
+    };
+    // point p = 8 c + e at LDS row 8 c + (e ^ bit 1 of c), its halves of 64 bytes exchanged where c is odd: the four groups of lanes, whose c differ in both
+    // bits, read from all banks
+    const uint32_t code_k = (uint32_t)k0 + (((lane & 7) ^ ((wave & 1) << 2)) << 4);
+    const uint32_t code_at = (uint32_t)(wave * 8 + ((lane >> 3) ^ (wave >> 1))) * stride + (code_k < stride ? code_k : kOutside);
+    auto copy_codes = [&](uint32_t step, uint32_t stage) {
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, (__attribute__((address_space(3))) void*)(lds + CODES + stage * kTurnStage + (q * 4 + wave) * 1024), 16,
+                                                     (int)code_at, (int)(step < steps ? (step * kStep + q * 32) * stride : kPast), 0, 0);
+        // (each wave its own, or the waves would not wait for the same number of copies)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(lds + SCALES + (stage * 4 + wave) * 256), 4, lane * 4, (int)(step < steps ? step * kStep : 0), 0, 0);
+    };
+    // ---- the codes: from LDS, then two points at a time to bf16
+    using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+    const uint32_t from_even = mine * 1024 + ((mine >> 1) & 1) * 128 + ((side ^ (mine & 1)) << 6) + (lane & 15) * 4, from_odd = from_even - ((mine >> 1) & 1) * 256;
+    uint32_t code[8];
+    u32x2 bytes;
+    auto read_codes = [&](uint32_t stage) {
+        const uint8_t* at = lds + CODES + stage * kTurnStage;
+#pragma unroll
+        for (int e = 0; e < 8; e++) code[e] = *reinterpret_cast<const uint32_t*>(at + (e & 1 ? from_odd : from_even) + e * 128);
+        bytes = *reinterpret_cast<const u32x2*>(lds + SCALES + (stage * 4 + wave) * 256 + mine * 8);
+    };
+    u32x4 frag[2][4];   // [step's parity][coordinate 4 (lane & 15) + f]: 8 points
+    auto widen = [&](int pair, u32x4 (&to)[4]) {
+        uint32_t w[2][2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int at = pair * 2 + e;
+            const float scale = __uint_as_float(((bytes[at >> 2] >> ((at & 3) * 8)) & 255u) << 23);
+            w[e][0] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[at], scale, false));
+            w[e][1] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[at], scale, true));
+        }
+#pragma unroll
+        for (int f = 0; f < 4; f++) to[f][pair] = __builtin_amdgcn_perm(w[1][f >> 1], w[0][f >> 1], f & 1 ? 0x07060302u : 0x05040100u);
+    };
+    // ---- the rows: fragment by fragment, read two ahead
+    const uint32_t row_at = (lane & 15) * 128 + ((mine ^ turn<8>(lane & 15)) << 4);
+    u32x4 rows[4];
+    f32x4 acc[FR][4];
+#pragma unroll
+    for (int i = 0; i < FR; i++)
+#pragma unroll
+        for (int f = 0; f < 4; f++) acc[i][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    uint32_t stage = 0;   // of this step
+    auto step = [&](uint32_t t, auto which, auto last) {
+        constexpr int S = decltype(which)::value;
+        constexpr bool LAST = decltype(last)::value;
+        const uint32_t next = stage == 2 ? 0 : stage + 1;
+#pragma unroll
+        for (int i = 0; i < FR; i++) {
+            if (!LAST && i == FR - 1) read_codes(next == 2 ? 0 : next + 1);
+            if (!LAST && i == FR - 2) {
+                // The step's rows and the next one's codes have been read by everybody; the next one's rows and the codes after them have to be there,
+                // the copies of one step may be on their way.
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COPIES) : "memory");
+                __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                copy_dc(t + 3, stage);
+                copy_codes(t + 4, next);
+            }
+            if (i + 2 < FR) rows[(S * FR + i + 2) & 3] = *reinterpret_cast<const u32x4*>(lds + stage * STAGE + row_at + (i + 2) * 2048);
+            else if (!LAST) rows[(S * FR + i + 2) & 3] = *reinterpret_cast<const u32x4*>(lds + next * STAGE + row_at + (i + 2 - FR) * 2048);
+            __builtin_amdgcn_sched_barrier(0);
+            bf16x8 v = __builtin_bit_cast(bf16x8, rows[(S * FR + i) & 3]);
+            if constexpr (LAST) {   // cut what lies behind the last point
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = t * kStep + mine * 8 + e < points ? v[e] : (__bf16)0.f;
+            }
+#pragma unroll
+            for (int f = 0; f < 4; f++) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, frag[S][f]), v, acc[i][f], 0, 0, 0);
+            if (!LAST) {
+#pragma unroll
+                for (int pair = 0; pair < 4; pair++)
+                    if (i == pair * (FR - 1) / 4) widen(pair, frag[S ^ 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        stage = next;
+    };
+    uint32_t t = 0u - (steps & 1);   // an odd number of steps begins with one of zeros
+    copy_codes(t, 0);
+    copy_dc(t, 0);
+    copy_codes(t + 1, 1);
+    copy_dc(t + 1, 1);
+    copy_codes(t + 2, 2);
+    copy_dc(t + 2, 2);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 + 2 * COPIES_DC) : "memory");   // (of the second step's rows and behind)
+    __syncthreads();
+    read_codes(0);
+#pragma unroll
+    for (int pair = 0; pair < 4; pair++) widen(pair, frag[0]);
+    rows[0] = *reinterpret_cast<const u32x4*>(lds + row_at);
+    rows[1] = *reinterpret_cast<const u32x4*>(lds + row_at + 2048);
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    copy_codes(t + 3, 0);
+    read_codes(1);
+    constexpr std::integral_constant<int, 0> even;
+    constexpr std::integral_constant<int, 1> odd;
+    for (; t + 2 != steps; t += 2) {
+        step(t, even, std::false_type{});
+        step(t + 1, odd, std::false_type{});
+    }
+    step(t, even, std::false_type{});
+    step(t + 1, odd, std::true_type{});
+    // ---- the two halves of the points, through LDS (the copies for nobody have ended first)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    f32x4* meet = reinterpret_cast<f32x4*>(lds) + side * (FR * 4 * 64) + lane;
+    if (half) {
+#pragma unroll
+        for (int i = 0; i < FR; i++)
+#pragma unroll
+            for (int f = 0; f < 4; f++) meet[(i * 4 + f) * 64] = acc[i][f];
+    }
+    __syncthreads();
+    if (!half) {
+#pragma unroll
+        for (int i = 0; i < FR; i++)
+#pragma unroll
+            for (int f = 0; f < 4; f++) acc[i][f] += meet[(i * 4 + f) * 64];
+    }
+    __syncthreads();
+    // ---- out, row by row: lane (i, g) holds rows i of the fragments, coordinates 16 g + 4 e + f of the wave's 64 in acc[.][f][e]
+    constexpr int OUT = kBlock * 4 + 16;   // (neighbours start 4 banks apart)
+    if (!half) {
+        uint8_t* to = lds + (lane & 15) * OUT + side * 256 + g * 64;
+#pragma unroll
+        for (int i = 0; i < FR; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) *reinterpret_cast<f32x4*>(to + i * 16 * OUT + e * 16) = f32x4{acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (uint32_t r = tid >> 5; r < mi; r += 8) put(a, slice, i0 + r, k0 + (tid & 31) * 4, *reinterpret_cast<const f32x4*>(lds + r * OUT + (tid & 31) * 16));
 }
 
 // The slices' sums in order: 256 / GROUPS runs of 4 coordinates a workgroup, GROUPS threads for each, whose shares of the slices are added last.
@@ -244,13 +453,14 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const float* __restrict_
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
     if (u < m * quads) {
         const float* from = part + u * 4;
+#pragma unroll 8
         for (uint32_t q = b; q < e; q++) s += *reinterpret_cast<const f32x4*>(from + q * (m * ldp));
     }
     if constexpr (GROUPS > 1) {
         sum[threadIdx.x] = s;
         __syncthreads();
         if (group) return;
-#pragma unroll
+#pragma unroll 4
         for (int g = 1; g < GROUPS; g++) s += sum[g * RUNS + threadIdx.x];
     }
     if (u >= m * quads) return;
@@ -261,35 +471,44 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const float* __restrict_
 }
 
 struct GradPlan {
-    uint32_t fr;
+    uint32_t fr;   // 64 rows of dc a tile, or 128
     uint64_t tiles_m, tiles_k, slices, per_slice, ldp, bytes;
 };
 GradPlan grad_plan(uint64_t m, uint64_t n, uint64_t dim, uint32_t dctype) {
-    GradPlan g;
-    // 128 rows read the points half as often as 64 (300 x 60 000 x 784 of bf16: 52 against 67 us, 1024 rows: 127 against 189); more of them, or 128 of
-    // f32, leave one workgroup on a CU, whose waits nothing fills (256 rows: 73 and 135 us; f32, 128 rows: 165 against 116 us)
-    g.fr = m > 64 && dctype != AE_TYPE_F32 ? 2 : 1;
-    g.tiles_m = (m + 64 * g.fr - 1) / (64 * g.fr);
-    g.tiles_k = (dim + kBlock - 1) / kBlock;
-    const uint64_t resident = 512;   // two workgroups on each of 256 CUs
-    const uint64_t steps = (n + kStep - 1) / kStep, tiles = g.tiles_m * g.tiles_k;
-    uint64_t want = tiles >= resident ? 1 : resident / tiles;
-    if (want > (steps + 3) / 4) want = (steps + 3) / 4;
+    GradPlan best{};
+    const uint64_t steps = std::max<uint64_t>((n + kStep - 1) / kStep, 1), tiles_k = (dim + kBlock - 1) / kBlock, ldp = (dim + 3) / 4 * 4;
     const uint64_t most = 0x3FFF0000ull / points8_row_bytes(dim) / kStep, least_slices = (steps + most - 1) / most;   // a slice's codes: less than 1 GiB
-    if (want < least_slices) want = least_slices;
-    if (want < 1) want = 1;
-    const uint64_t per = (steps + want - 1) / want;
-    g.per_slice = per * kStep;
-    g.slices = steps ? (steps + per - 1) / per : 1;
-    g.ldp = (dim + 3) / 4 * 4;
-    g.bytes = g.slices * m * g.ldp * 4;
-    return g;
+    // What a choice costs, in us: a workgroup's beginning and end; its steps, with so many workgroups on a CU (measured at 300 x 60 000 x 784 in 7, 14 and 22
+    // slices of 64 rows and 12 and 24 of 128; more rows of f32, more workgroups of f16 and f32 do not fit); the slices' sums, written and read again at 5
+    // TB/s; the launch that joins them.  300 x 60 000 x 784 of bf16 takes 49 us as chosen, 49 to 60 with the other choices; 1024 rows 107 against 126 to
+    // 181; 1000 x 1000 x 1000 in one slice 12.6 against 16 to 21 in several.
+    struct Choice { uint32_t fr, wgs; float step; };
+    static constexpr Choice bf16[] = {{1, 1, 0.41f}, {1, 2, 0.57f}, {1, 3, 0.84f}, {2, 1, 0.51f}, {2, 2, 0.82f}};
+    static constexpr Choice f16[] = {{1, 1, 0.84f}, {1, 2, 1.1f}, {2, 1, 1.25f}, {2, 2, 1.76f}};
+    static constexpr Choice f32[] = {{1, 1, 1.07f}, {1, 2, 1.46f}};
+    const Choice* const choices = dctype == AE_TYPE_BF16 ? bf16 : dctype == AE_TYPE_F16 ? f16 : f32;
+    const int count = dctype == AE_TYPE_BF16 ? 5 : dctype == AE_TYPE_F16 ? 4 : 2;
+    double least = 0.;
+    for (int q = 0; q < count; q++) {
+        const Choice& c = choices[q];
+        const uint64_t tiles_m = (m + 64 * c.fr - 1) / (64 * c.fr), tiles = tiles_m * tiles_k, slots = 256 * c.wgs;
+        for (const uint64_t want : {(uint64_t)1, slots / tiles}) {
+            const uint64_t slices = std::max<uint64_t>({1, least_slices, std::min(want, (steps + 3) / 4)}), per = (steps + slices - 1) / slices, used = (steps + per - 1) / per;
+            const double rounds = (double)((tiles * used + slots - 1) / slots);
+            const double cost = rounds * ((c.fr == 1 ? 2 : 6) + per * c.step) + (used > 1 ? 4. + used * (0.005 + m * ldp * 8 / 5.1e6) : 0.);
+            if (best.fr && cost >= least) continue;
+            least = cost;
+            best = GradPlan{c.fr, tiles_m, tiles_k, used, per * kStep, ldp, used > 1 ? used * m * ldp * 4 : 0};
+        }
+    }
+    return best;
 }
 
 template <int TYPE, int FR>
 void launch_grad(const GradArgs& a, bool vec, unsigned grid, hipStream_t s) {
-    if (vec) hipLaunchKernelGGL((grad_tile_kernel<TYPE, FR, true>), dim3(grid), dim3(256), (grad_lds<TYPE, FR>()), s, a);
-    else hipLaunchKernelGGL((grad_tile_kernel<TYPE, FR, false>), dim3(grid), dim3(256), (grad_lds<TYPE, FR>()), s, a);
+    if (!vec) hipLaunchKernelGGL((grad_tile_kernel<TYPE, FR, false>), dim3(grid), dim3(256), (grad_lds<TYPE, FR>()), s, a);
+    else if constexpr (TYPE == AE_TYPE_BF16) hipLaunchKernelGGL((grad_turn_kernel<4 * FR>), dim3(grid), dim3(256), (turn_lds<4 * FR>()), s, a);
+    else hipLaunchKernelGGL((grad_tile_kernel<TYPE, FR, true>), dim3(grid), dim3(256), (grad_lds<TYPE, FR>()), s, a);
 }
 
 }  // namespace
@@ -321,13 +540,13 @@ int32_t ae_points8_product_grad(const ae_points8* p, uint64_t first, uint64_t n,
         if (g.bytes && (!d_work || work_bytes < g.bytes))
             fail(AE_ERR_INVALID_ARG, "ae_points8_product_grad: %llu bytes of scratch are needed, %llu given", (unsigned long long)g.bytes, (unsigned long long)work_bytes);
         check_aligned(d_work, 16, "ae_points8_product_grad: work");
-        const unsigned groups = g.slices >= 64 ? 16 : g.slices >= 8 ? 4 : 1;   // (the join's)
+        const unsigned groups = g.slices >= 192 ? 64 : g.slices >= 48 ? 16 : g.slices >= 8 ? 4 : 1;   // (the join's)
         const uint64_t runs = m * (g.ldp / 4);
         if (g.tiles_m * g.tiles_k * g.slices > 0x3FFFFFull || runs * groups > 0xFFFF0000ull)
             fail(AE_ERR_INVALID_ARG, "ae_points8_product_grad: %llu rows are more than one call takes", (unsigned long long)m);
         if (n) {
             const uint64_t tiles = g.tiles_m * g.tiles_k;
-            GradArgs a{d_dc, lddc, m, n, p->dim, points8_rows(p, first, n), g.per_slice, (float*)d_work, g.ldp, (uint32_t)g.tiles_k, (uint32_t)tiles, (uint32_t)g.slices};
+            GradArgs a{d_dc, lddc, m, n, p->dim, points8_rows(p, first, n), g.per_slice, (float*)d_work, g.ldp, (uint32_t)g.tiles_k, (uint32_t)tiles, (uint32_t)g.slices, d_dx, xtype, lddx};
             const unsigned grid = (unsigned)((tiles * g.slices + 7) / 8 * 8);
             // The copies take 16 bytes at any address and the dwords that the buffer's range holds whole.  The last of an odd number of 16-bit values is the
             // first half of a dword: the range then goes 2 bytes past it, which must not be the next page.
@@ -339,6 +558,7 @@ int32_t ae_points8_product_grad(const ae_points8* p, uint64_t first, uint64_t n,
                 else if constexpr (TYPE != AE_TYPE_F32) launch_grad<TYPE, 2>(a, vec, grid, s);
             });
             check_launch("points8_product_grad");
+            if (g.slices == 1) return;
         }
         by_type(xtype, [&](auto ty) {
             constexpr int TYPE = decltype(ty)::value;
@@ -346,7 +566,8 @@ int32_t ae_points8_product_grad(const ae_points8* p, uint64_t first, uint64_t n,
                 hipLaunchKernelGGL(kernel, dim3(blocks_for(runs * groups, 256)), dim3(256), 0, s, (const float*)d_work, (uint32_t)g.slices, m, p->dim, g.ldp,
                                    static_cast<typename Elem<TYPE>::T*>(d_dx), lddx);
             };
-            if (groups == 16) go(grad_join_kernel<TYPE, 16>);
+            if (groups == 64) go(grad_join_kernel<TYPE, 64>);
+            else if (groups == 16) go(grad_join_kernel<TYPE, 16>);
             else if (groups == 4) go(grad_join_kernel<TYPE, 4>);
             else go(grad_join_kernel<TYPE, 1>);
         });

@@ -315,7 +315,7 @@ def test_refusals(A):
         lambda: bank.product(x[:, :60]), lambda: bank.product(x, n=101), lambda: bank.product(x.repeat(3, 1), work=torch.zeros(3, device="cuda")),
         lambda: bank.product(x, out=torch.zeros(10, 99, device="cuda")), lambda: bank.product(A.Points8(5, 32)), lambda: bank.product(A.Points8(5, 64), m=6),
         lambda: bank.product_grad(x), lambda: bank.product_grad(torch.zeros(4, 100, device="cuda", dtype=torch.int32)),
-        lambda: bank.product_grad(torch.zeros(4, 100, device="cuda"), work=torch.zeros(1, device="cuda")),
+        lambda: A.Points8(5000, 64).product_grad(torch.zeros(4, 5000, device="cuda"), work=torch.zeros(1, device="cuda")),
         lambda: A.KGraph.bruteforce_l2_points8(bank, 0), lambda: A.KGraph.bruteforce_l2_points8(bank, 10, n=10), lambda: A.KGraph.bruteforce_l2_points8(bank, 3, n=200),
     ]
     for f in bad:
