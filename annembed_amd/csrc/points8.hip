@@ -12,7 +12,9 @@ namespace {
 
 constexpr int kGroups = 16;    // blocks per workgroup and trip
 constexpr int kTrips = 4;      // blocks a group has in flight: 64 to 128 bytes of loads per lane
-constexpr uint32_t kScan = 1024;   // up to this many slots a row looks for a later occurrence of its slot itself
+// Up to this many slots a workgroup looks for later occurrences of its rows' slots itself, in one launch: 4096 rows of 128 take 6.9 us against 8.0 of
+// the two or three launches otherwise, 5000 of 784 7.3 against 11.1; 8191 of 128 10.1 against 8.0, 8000 of 1500 18.4 against 16.0.
+constexpr uint32_t kScan = 6000;
 
 struct Blocks {   // the call's blocks
     uint64_t units, n;
@@ -47,21 +49,21 @@ __global__ void __launch_bounds__(256) points8_release_kernel(const uint32_t* __
     if (s < capacity) owner[s] = 0;
 }
 
-// SLOTS 0: row i to first + i.  1: to slots[i], each row scans for a later row of the same slot.  2: to slots[i] where owner says so.  3: the same
+// SLOTS 0: row i to first + i.  1: to slots[i], unless a later row has the same slot.  2: to slots[i] where owner says so.  3: the same
 // for rows of one block, which give their slot back themselves (another row of that slot finds the owner or nobody: not itself).
-template <int TYPE, int SLOTS>
+template <int TYPE, int SLOTS, int TRIPS>
 __global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<TYPE>::T* __restrict__ x, uint64_t ldx, uint64_t dim, Blocks bl, uint64_t first,
                                                             const uint32_t* __restrict__ slots, uint32_t* __restrict__ owner, uint64_t capacity,
                                                             uint8_t* __restrict__ codes, uint64_t row_bytes, uint8_t* __restrict__ scales, uint64_t scale_stride) {
-    const uint64_t u0 = blockIdx.x * (uint64_t)(kGroups * kTrips);
+    const uint64_t u0 = blockIdx.x * (uint64_t)(kGroups * TRIPS);
     const Cursor cur(u0, bl.nb);
     const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
-    float v[kTrips][8];
-    uint64_t row[kTrips];
-    uint32_t b[kTrips];
-    bool live[kTrips];
+    float v[TRIPS][8];
+    uint64_t row[TRIPS];
+    uint32_t b[TRIPS];
+    bool live[TRIPS];
 #pragma unroll
-    for (int t = 0; t < kTrips; t++) {
+    for (int t = 0; t < TRIPS; t++) {
         const uint32_t off = t * kGroups + group;
         cur.at(off, bl.nb, row[t], b[t]);
         live[t] = u0 + off < bl.units;
@@ -69,8 +71,47 @@ __global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<
         const int count = !live[t] || k >= dim ? 0 : (int)min((uint64_t)8, dim - k);
         load8<TYPE>(x + (count ? row[t] * ldx + k : 0), count, v[t]);
     }
+    __shared__ uint8_t later[kGroups * TRIPS];   // rows of this workgroup whose slot comes again
+    if constexpr (SLOTS == 1) {   // all slots pass by once, four a thread, and are compared with those of the workgroup's rows
+        const uint32_t n = (uint32_t)bl.n, first_row = (uint32_t)cur.row0, rows = min(n - first_row, (cur.rem0 + kGroups * TRIPS - 1) / bl.nb + 1);
+        __shared__ __attribute__((aligned(16))) uint32_t mine[kGroups * TRIPS];
+        if (threadIdx.x < kGroups * TRIPS) {
+            later[threadIdx.x] = 0;
+            mine[threadIdx.x] = threadIdx.x < rows ? slots[first_row + threadIdx.x] : 0xFFFFFFFFu;
+        }
+        __syncthreads();
+        for (uint32_t c = (first_row + 1) & ~1023u; c < n; c += 1024) {
+            const uint32_t j = c + threadIdx.x * 4;
+            uint32_t s[4];
+            if (j + 4 <= n) {
+                const Piece four = *reinterpret_cast<const Piece*>(slots + j);
 #pragma unroll
-    for (int t = 0; t < kTrips; t++) {
+                for (int e = 0; e < 4; e++) s[e] = four[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[e] = j + e < n ? slots[j + e] : 0xFFFFFFFFu;   // (no row's that is written)
+            }
+            for (uint32_t r = 0; r < rows; r += 4) {
+                const u32x4 to = *reinterpret_cast<const u32x4*>(mine + r);
+                uint32_t again = 0;   // bit q: row r + q
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    uint32_t last = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) last = s[e] == to[q] ? j + e : last;
+                    again |= last > first_row + r + q ? 1u << q : 0u;
+                }
+                if (again) {   // (rarely)
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        if (again >> q & 1) later[r + q] = 1;
+                }
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < TRIPS; t++) {
         const uint32_t byte = scale_byte(max16(amax8(v[t])));
         uint64_t to = first + row[t];
         if constexpr (SLOTS != 0) {
@@ -81,13 +122,7 @@ __global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<
                 if constexpr (SLOTS >= 2) live[t] = live[t] && owner[s] == (uint32_t)row[t] + 1;
                 if constexpr (SLOTS == 3) { if (live[t] && lane == 0) owner[s] = 0; }
             }
-            if constexpr (SLOTS == 1) {
-                bool later = false;
-                if (live[t])
-                    for (uint64_t j = row[t] + 1 + lane; j < bl.n; j += 16) later |= slots[j] == (uint32_t)to;
-                const uint64_t seen = __ballot(later);
-                live[t] = live[t] && ((seen >> (threadIdx.x & 48)) & 0xFFFFull) == 0;
-            }
+            if constexpr (SLOTS == 1) live[t] = live[t] && !later[row[t] - cur.row0];
         }
         const uint64_t k = b[t] * (uint64_t)kBlock + lane * 8;
         if (live[t] && k < row_bytes) *reinterpret_cast<uint2*>(codes + to * row_bytes + k) = encode8(v[t], byte);
@@ -149,21 +184,21 @@ Blocks blocks_of(uint64_t n, uint64_t dim) {
     bl.units = n * bl.nb;
     return bl;
 }
-unsigned trips_grid(const Blocks& bl) {
-    const uint64_t g = (bl.units + kGroups * kTrips - 1) / (kGroups * kTrips);
+unsigned trips_grid(const Blocks& bl, int trips) {
+    const uint64_t g = (bl.units + kGroups * trips - 1) / (kGroups * trips);
     if (g * 256 > 0xFFFFFFFFull) fail(AE_ERR_INVALID_ARG, "%llu rows of %u blocks are more than one call takes", (unsigned long long)bl.n, bl.nb);
     return (unsigned)g;
 }
 
-template <int SLOTS>
+template <int SLOTS, int TRIPS = kTrips>
 void launch_write(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint64_t first, const uint32_t* slots, uint32_t* owner, uint64_t capacity,
                   uint8_t* codes, uint8_t* scales, uint64_t scale_stride, hipStream_t s) {
     const Blocks bl = blocks_of(n, dim);
-    const unsigned grid = trips_grid(bl);
+    const unsigned grid = trips_grid(bl, TRIPS);
     by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         const auto* x = static_cast<const typename Elem<TYPE>::T*>(d_x);
-        hipLaunchKernelGGL((points8_write_kernel<TYPE, SLOTS>), dim3(grid), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales,
+        hipLaunchKernelGGL((points8_write_kernel<TYPE, SLOTS, TRIPS>), dim3(grid), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales,
                            scale_stride);
     });
     check_launch("points8_write");
@@ -171,7 +206,7 @@ void launch_write(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint
 
 void read_rows(const ae_points8* p, uint64_t first, const uint32_t* slots, uint64_t n, void* d_x, uint32_t type, uint64_t ldx, hipStream_t s) {
     const Blocks bl = blocks_of(n, p->dim);
-    const unsigned grid = trips_grid(bl);
+    const unsigned grid = trips_grid(bl, kTrips);
     by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         auto* x = static_cast<typename Elem<TYPE>::T*>(d_x);
@@ -263,10 +298,13 @@ int32_t ae_points8_write(ae_points8* p, const void* d_x, uint32_t type, uint64_t
         }
         check_aligned(d_slots, 4, "ae_points8_write: slots");
         if (n > 0x7FFFFFFFull) fail(AE_ERR_INVALID_ARG, "ae_points8_write: %llu slots are more than one call takes", (unsigned long long)n);
-        // The last row of a repeated slot is held.  Few rows: every block scans the slots behind its own, one launch.  More: the rows claim
+        // The last row of a repeated slot is held.  Few rows: every workgroup looks at the slots behind its own, one launch.  More: the rows claim
         // their slots first and give them back as they are written, or, rows of several blocks, in a launch of their own.
         if (n <= kScan) {
-            launch_write<1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
+            // one block a group of lanes spreads few rows over more workgroups (4096 rows of 128: 6.9 against 20 us with four), but each of them looks
+            // at all slots (4096 rows of 4096: 18.5 against 16.2)
+            if (n * p->blocks <= 65536) launch_write<1, 1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
+            else launch_write<1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
             return;
         }
         const unsigned grid = blocks_for(n, 256);

@@ -15,6 +15,7 @@ allocate outside torch's allocator, so they can be captured into a graph.  The f
 ae_teacher_* in include/annembed_hip.h.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -80,11 +81,28 @@ def _call(device, fn, *args):
             check(f(*args, _stream(device.index)))
 
 
+@functools.lru_cache(maxsize=1024)
+def _loss_work(rows, cols):
+    """bytes of scratch, asked for once for each size"""
+    need = C.c_uint64()
+    check(L.load().ae_teacher_loss_work(rows, cols, C.byref(need)))
+    return need.value
+
+
 class _Store:
-    """the handle; views of its memory keep it alive"""
+    """the handle, and the bytes of scratch of its calls, asked for once for each size; views of its memory keep it alive"""
 
     def __init__(self, h):
+        def asked(fn):
+            @functools.lru_cache(maxsize=1024)
+            def need(*sizes):
+                bytes_ = C.c_uint64()
+                check(fn(h, *sizes, C.byref(bytes_)))
+                return bytes_.value
+            return need
+
         self.h = h
+        self.product_work, self.product_grad_work = asked(L.load().ae_points8_product_work), asked(L.load().ae_points8_product_grad_work)
 
     def __del__(self):
         try:
@@ -191,9 +209,7 @@ class Points8:
         if isinstance(x, Points8):
             _call(self.device, "ae_points8_product_points", self._store.h, first, n, x._store.h, x_first, m, p, ty, ld)
             return out
-        need = C.c_uint64()
-        check(L.load().ae_points8_product_work(self._store.h, n, m, C.byref(need)))
-        wp, wn, keep = self._work(work, need.value)
+        wp, wn, keep = self._work(work, self._store.product_work(n, m))
         _call(self.device, "ae_points8_product", self._store.h, first, n, xp, xt, m, xl, p, ty, ld, wp, wn)
         return out
 
@@ -207,29 +223,27 @@ class Points8:
         if out is None:
             out = torch.empty(m, self.dim, dtype=dtype, device=self.device)
         p, ty, ld = _rows(out, "out", self.device, (m, self.dim))
-        need = C.c_uint64()
-        check(L.load().ae_points8_product_grad_work(self._store.h, n, m, dt, C.byref(need)))
-        wp, wn, keep = self._work(work, need.value)
+        wp, wn, keep = self._work(work, self._store.product_grad_work(n, m, dt))
         _call(self.device, "ae_points8_product_grad", self._store.h, first, n, dp, dt, m, dl, p, ty, ld, wp, wn)
         return out
 
 
 def _list(idx, values, rows, device):
     """pointers, length and stride of a teacher's lists [rows, k]"""
-    if not isinstance(idx, torch.Tensor) or idx.dim() != 2 or idx.shape[0] != rows or idx.dtype not in _INDEX:
+    if not isinstance(idx, torch.Tensor) or idx.dim() != 2 or idx.dtype not in _INDEX or idx.shape[0] != rows:
         raise _bad("idx has to be an int32 tensor of %d rows" % rows)
     if not isinstance(values, torch.Tensor) or values.shape != idx.shape or values.dtype != torch.float32:
         raise _bad("the list's values have to be a float32 tensor of idx's shape")
     if idx.device != device or values.device != device:
         raise _bad("the lists are on %s and %s, not on %s" % (idx.device, values.device, device))
-    k = idx.shape[1]
+    k, (ld, inner), theirs = idx.shape[1], idx.stride(), values.stride()
     if rows <= 1:
-        if k > 1 and (idx.stride(1) != 1 or values.stride(1) != 1):
+        if k > 1 and (inner != 1 or theirs[1] != 1):
             raise _bad("the lists' entries have to be next to each other")
-        return idx.data_ptr(), values.data_ptr(), k, k
-    if idx.stride() != values.stride() or (k > 1 and idx.stride(1) != 1) or idx.stride(0) < k:
+        ld = k
+    elif (ld, inner) != theirs or (k > 1 and inner != 1) or ld < k:
         raise _bad("idx and the list's values have to have the same strides, entries next to each other")
-    return idx.data_ptr(), values.data_ptr(), k, idx.stride(0)
+    return idx.data_ptr(), values.data_ptr(), k, ld
 
 
 def _kind(teacher):
@@ -266,11 +280,10 @@ def teacher_loss(logits, idx, values, teacher="proba", temperature=1.0, row_weig
         gp, gt, gl = _rows(g, "grad", device, (rows, cols))
         if gt != ty:
             raise _bad("grad is %s, the logits %s" % (g.dtype, logits.dtype))
-    need = C.c_uint64()
-    check(L.load().ae_teacher_loss_work(rows, cols, C.byref(need)))
-    if work is None and need.value:
-        work = torch.empty(need.value, dtype=torch.uint8, device=device)
-    if work is not None and (not isinstance(work, torch.Tensor) or work.device != device or not work.is_contiguous()):
+    need = _loss_work(rows, cols)
+    if work is None:
+        work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    elif not isinstance(work, torch.Tensor) or work.device != device or not work.is_contiguous():
         raise _bad("work has to be a contiguous tensor on %s" % device)
     _call(device, "ae_teacher_loss", p, ty, rows, cols, ld, ip, vp, k, ldk, _kind(teacher), float(temperature), wp, loss.data_ptr(), stats.data_ptr(), gp, gl,
           None if work is None else work.data_ptr(), 0 if work is None else work.numel() * work.element_size())

@@ -635,7 +635,7 @@ int32_t ae_points8_product_work(const ae_points8 *p, uint64_t n, uint64_t m, uin
 int32_t ae_points8_product_points(const ae_points8 *p, uint64_t first, uint64_t n, const ae_points8 *q, uint64_t q_first, uint64_t m,
                                   void *d_c, uint32_t ctype, uint64_t ldc, void *stream);
 /* The gradient of ae_points8_product to its rows, q taken as the identity: dx[i][k] = sum_j dc[i][j] * p_{first + j}[k].  dc enters exactly
-   whatever its type (but for what lies below 2^-126), sums are f32 in an order that depends on the sizes only. */
+   whatever its type (but for what lies below 2^-126), sums are f32 in an order that equal calls share. */
 int32_t ae_points8_product_grad(const ae_points8 *p, uint64_t first, uint64_t n, const void *d_dc, uint32_t dctype, uint64_t m,
                                 uint64_t lddc, void *d_dx, uint32_t xtype, uint64_t lddx, void *d_work, uint64_t work_bytes, void *stream);
 int32_t ae_points8_product_grad_work(const ae_points8 *p, uint64_t n, uint64_t m, uint32_t dctype, uint64_t *bytes);

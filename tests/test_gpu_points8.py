@@ -415,3 +415,22 @@ def test_rows_behind_the_last_point_do_not_count(A):
             wide[1:-1, 5:25] = dc.cuda()
             got, want = n64(bank.product_grad(wide[1:-1, 5:25], n=20, first=16)), n64(dc) @ pv
             assert (np.abs(got - want) <= product_bound(n64(dc), pv, 3 * 20 + 64, want, torch.float32)).all()
+
+
+@pytest.mark.parametrize("n,dim", [(4097, 40), (6000, 100), (6001, 100), (6000, 1500), (6001, 784)])
+def test_slots_that_come_again_far_behind(A, n, dim):
+    """repeated slots at every distance, on both sides of the number of rows up to which a workgroup looks for them itself"""
+    cap = n // 3
+    bank = A.Points8(cap, dim)
+    x = vectors(n, dim, 5)
+    rng = np.random.default_rng(n)
+    slots = rng.integers(0, cap, n)
+    slots[rng.random(n) < 0.1] = -1
+    slots[0] = slots[n - 1] = 7
+    bank.write(x.cuda(), slots=torch.from_numpy(slots).to(torch.int32).cuda())
+    last = {s: i for i, s in enumerate(slots.tolist()) if s >= 0}
+    at = sorted(last)
+    v = U.values(n64(x[[last[s] for s in at]]))
+    np.testing.assert_array_equal(n64(bank.read(slots=torch.tensor(at, dtype=torch.int32, device="cuda"))), v)
+    rest = sorted(set(range(cap)) - set(at))
+    assert not bank.read(slots=torch.tensor(rest, dtype=torch.int32, device="cuda")).any()
