@@ -340,14 +340,19 @@ void product(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t c
     else launch_tiles<128, 128, 64>(x, p, dim, d_c, ctype, ldc, s);
 }
 
-// Up to 16 rows: bound by the points' bytes, which go from memory straight to the matrix cores (16 points a wave, 32 coordinates of a block
+// Few rows: bound by the points' bytes, which go from memory straight to the matrix cores (16 points a wave, 32 coordinates of a block
 // a lane).  Every workgroup quantises the rows itself, into LDS as the bf16 values they stand for, while its first points are on their way: one
 // launch.  SPLIT waves share the blocks of a group of points where there are few points.
-constexpr int kFew = 16;
+constexpr int kFew = 64;
 constexpr uint64_t few_lds_row(uint64_t dim) { return ((dim + kBlock - 1) / kBlock * kBlock) * 2 + 16; }   // (16 bytes more: neighbours start 4 banks apart)
-bool few_rows(uint64_t m, uint64_t n, uint64_t dim) { return m <= kFew && m * few_lds_row(dim) <= 48 * 1024 && n < 1ull << 30; }   // (64 points, 256 threads: below 2^32)
+// From 17 rows on while the products are few: every workgroup's own quantising and the exact bf16 products cost more than a second launch then (32 x 2000 x 300
+// of f32: 7.8 against 11.3 us; 17 x 60 000 x 128: 8.6 against 10.3; 17 x 20 000 x 700: 14.6 against 13.7; 48 x 60 000 x 128: 17.0 against 11.7).
+bool few_rows(uint64_t m, uint64_t n, uint64_t dim) {
+    if (m > kFew || m * few_lds_row(dim) > 48 * 1024 || n >= 1ull << 30) return false;   // (64 points, 256 threads: fewer than 2^32)
+    return m <= 16 || (m * n <= 1 << 20 && m * n * dim <= 200000000);
+}
 
-template <int XTYPE, int SPLIT>
+template <int XTYPE, int SPLIT, int TILES>   // TILES of 16 rows
 __global__ void __launch_bounds__(256) product_few_kernel(const typename Elem<XTYPE>::T* __restrict__ x, uint32_t m, uint64_t ldx, uint32_t dim, Rows8 p, void* c_, uint32_t ctype, uint64_t ldc) {
     constexpr int GROUPS = 4 / SPLIT, AHEAD = 4;   // groups of 16 points a workgroup; blocks whose codes are fetched together
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -382,8 +387,13 @@ __global__ void __launch_bounds__(256) product_few_kernel(const typename Elem<XT
         *reinterpret_cast<bf16x8*>(lds + i * lds_row + k * 2) = widen8(e.x, e.y, scale);
     }
     __syncthreads();
-    const uint8_t* mine = lds + min((uint32_t)(lane & 15), m - 1) * lds_row + g * 64;   // (rows that do not exist repeat the last one, for nobody)
-    f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    uint32_t mine[TILES];   // (rows that do not exist repeat the last one, for nobody)
+    f32x4 acc[TILES][2];
+#pragma unroll
+    for (int i = 0; i < TILES; i++) {
+        mine[i] = min((uint32_t)(lane & 15) + i * 16, m - 1) * lds_row + g * 64;
+        acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     for (uint32_t kb = kb0; kb < blocks; kb += AHEAD * SPLIT) {
 #pragma unroll
         for (int q = 0; q < AHEAD; q++) {
@@ -391,38 +401,49 @@ __global__ void __launch_bounds__(256) product_few_kernel(const typename Elem<XT
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const bf16x8 wp = widen8(code[q][e >> 1][(e & 1) * 2], code[q][e >> 1][(e & 1) * 2 + 1], byte[q]);
-                const bf16x8 wx = *reinterpret_cast<const bf16x8*>(mine + at * (kBlock * 2) + e * 16);
-                acc[e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp, wx, acc[e & 1], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < TILES; i++) {
+                    const bf16x8 wx = *reinterpret_cast<const bf16x8*>(lds + mine[i] + at * (kBlock * 2) + e * 16);
+                    acc[i][e & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp, wx, acc[i][e & 1], 0, 0, 0);
+                }
             }
             load(kb + (q + AHEAD) * SPLIT, q);
         }
     }
-    f32x4 sum = acc[0] + acc[1];
+    f32x4 sum[TILES];
+#pragma unroll
+    for (int i = 0; i < TILES; i++) sum[i] = acc[i][0] + acc[i][1];
     if constexpr (SPLIT > 1) {   // the waves' shares in order
         __syncthreads();
         f32x4* part = reinterpret_cast<f32x4*>(lds);
-        part[tid] = sum;
+#pragma unroll
+        for (int i = 0; i < TILES; i++) part[i * 256 + tid] = sum[i];
         __syncthreads();
         if (wave % SPLIT) return;
 #pragma unroll
-        for (int q = 1; q < SPLIT; q++) sum += part[tid + q * 64];
-    }
-    // a lane holds 4 consecutive points of row lane & 15
-    const uint32_t i = lane & 15;
-    if (i >= m) return;
+        for (int i = 0; i < TILES; i++)
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const uint32_t j = g * 4 + e;
-        if (j >= nj) continue;
-        const uint64_t at = i * ldc + j0 + j;
-        if (ctype == AE_TYPE_F32) static_cast<float*>(c_)[at] = sum[e];
-        else if (ctype == AE_TYPE_BF16) static_cast<__bf16*>(c_)[at] = (__bf16)sum[e];
-        else static_cast<_Float16*>(c_)[at] = (_Float16)sum[e];
+            for (int q = 1; q < SPLIT; q++) sum[i] += part[i * 256 + tid + q * 64];
+    }
+    // a lane holds 4 consecutive points of rows lane & 15
+#pragma unroll
+    for (int i = 0; i < TILES; i++) {
+        const uint32_t r = i * 16 + (lane & 15);
+        if (r >= m) continue;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t j = g * 4 + e;
+            if (j >= nj) continue;
+            const uint64_t at = r * ldc + j0 + j;
+            if (ctype == AE_TYPE_F32) static_cast<float*>(c_)[at] = sum[i][e];
+            else if (ctype == AE_TYPE_BF16) static_cast<__bf16*>(c_)[at] = (__bf16)sum[i][e];
+            else static_cast<_Float16*>(c_)[at] = (_Float16)sum[i][e];
+        }
     }
 }
 
 void product_few(const void* d_x, uint32_t xtype, uint64_t m, uint64_t ldx, uint64_t dim, const Rows8& p, void* d_c, uint32_t ctype, uint64_t ldc, hipStream_t s) {
-    const unsigned bytes = (unsigned)std::max<uint64_t>(m * few_lds_row(dim), 4096);
+    const unsigned tiles = m <= 16 ? 1 : m <= 32 ? 2 : 4, bytes = (unsigned)std::max<uint64_t>(m * few_lds_row(dim), 4096 * tiles);
     by_type(xtype, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         auto go = [&](auto kernel, unsigned points) {
@@ -430,8 +451,10 @@ void product_few(const void* d_x, uint32_t xtype, uint64_t m, uint64_t ldx, uint
                                (uint32_t)dim, p, d_c, ctype, ldc);
         };
         // 16 points a wave leave half of the chip's waves without work below 32 768 points: four waves share them then
-        if (p.rows >= 32768 || points8_blocks(dim) < 4) go(product_few_kernel<TYPE, 1>, 64);
-        else go(product_few_kernel<TYPE, 4>, 16);
+        const bool whole = p.rows >= 32768 || points8_blocks(dim) < 4;
+        if (tiles == 1) whole ? go(product_few_kernel<TYPE, 1, 1>, 64) : go(product_few_kernel<TYPE, 4, 1>, 16);
+        else if (tiles == 2) whole ? go(product_few_kernel<TYPE, 1, 2>, 64) : go(product_few_kernel<TYPE, 4, 2>, 16);
+        else whole ? go(product_few_kernel<TYPE, 1, 4>, 64) : go(product_few_kernel<TYPE, 4, 4>, 16);
     });
     check_launch("points8_product_few");
 }

@@ -124,7 +124,7 @@ def product_bound(x, p, terms, want, dtype, eights=False):
     return (terms * 2.0 ** -23 + eights * 7 * 2.0 ** -13) * (np.abs(x) @ np.abs(p)) + f.eps / 2 * np.maximum(np.abs(want), f.smallest_normal)
 
 
-@pytest.mark.parametrize("m,n,dim", [(1, 1, 1), (1, 3, 28), (1, 1000, 784), (2, 129, 128), (5, 64, 130), (16, 500, 784), (17, 257, 100), (33, 31, 1000), (64, 2000, 16), (127, 128, 129),
+@pytest.mark.parametrize("m,n,dim", [(1, 1, 1), (1, 3, 28), (1, 1000, 784), (17, 33000, 28), (31, 700, 600), (50, 3000, 200), (64, 16384, 10), (2, 129, 128), (5, 64, 130), (16, 500, 784), (17, 257, 100), (33, 31, 1000), (64, 2000, 16), (127, 128, 129),
                                      (128, 128, 256), (129, 385, 640), (200, 1111, 784), (300, 700, 2000), (513, 1025, 64), (1, 40, 9000)])
 def test_product(A, m, n, dim):
     bank = A.Points8(n + 5, dim)
@@ -229,7 +229,7 @@ def test_offsets_past_32_bits(A):
     slots = torch.arange(cap - 300, cap, dtype=torch.int32, device="cuda")
     v = U.values(n64(x))
     np.testing.assert_array_equal(n64(bank.read(slots=slots)), v)
-    q = vectors(20, dim, 9)
+    q = vectors(70, dim, 9)
     qv = U.values(n64(q))
     got = n64(bank.product(q.cuda(), n=300, first=cap - 300))
     assert (np.abs(got - qv @ v.T) <= product_bound(qv, v.T, dim, qv @ v.T, torch.float32)).all()
@@ -312,7 +312,7 @@ def test_refusals(A):
         lambda: bank.write(x, slots=torch.zeros(9, dtype=torch.int32, device="cuda")), lambda: bank.write(x, slots=torch.zeros(10, dtype=torch.int64, device="cuda")),
         lambda: bank.write(x, slots=torch.zeros(10, dtype=torch.int32)), lambda: bank.read(n=101), lambda: bank.read(n=3, first=98),
         lambda: bank.read(dtype=torch.float64), lambda: bank.read(n=4, out=torch.zeros(5, 64, device="cuda")),
-        lambda: bank.product(x[:, :60]), lambda: bank.product(x, n=101), lambda: bank.product(x.repeat(3, 1), work=torch.zeros(3, device="cuda")),
+        lambda: bank.product(x[:, :60]), lambda: bank.product(x, n=101), lambda: bank.product(x.repeat(7, 1), work=torch.zeros(3, device="cuda")),
         lambda: bank.product(x, out=torch.zeros(10, 99, device="cuda")), lambda: bank.product(A.Points8(5, 32)), lambda: bank.product(A.Points8(5, 64), m=6),
         lambda: bank.product_grad(x), lambda: bank.product_grad(torch.zeros(4, 100, device="cuda", dtype=torch.int32)),
         lambda: A.Points8(5000, 64).product_grad(torch.zeros(4, 5000, device="cuda"), work=torch.zeros(1, device="cuda")),
@@ -329,8 +329,8 @@ def test_refusals(A):
     assert lib.ae_points8_write(None, x.data_ptr(), 0, 10, 64, 0, None, None) == L.AE_ERR_INVALID_ARG
     assert lib.ae_points8_write(bank.handle, x.data_ptr(), 0, 10, 63, 0, None, None) == L.AE_ERR_INVALID_ARG
     assert b"stride" in lib.ae_last_error_message()
-    many, c = x.repeat(3, 1), torch.zeros(30, 100, device="cuda")
-    assert lib.ae_points8_product(bank.handle, 0, 100, many.data_ptr(), 0, 30, 64, c.data_ptr(), 0, 100, None, 0, None) == L.AE_ERR_INVALID_ARG
+    many, c = x.repeat(7, 1), torch.zeros(70, 100, device="cuda")
+    assert lib.ae_points8_product(bank.handle, 0, 100, many.data_ptr(), 0, 70, 64, c.data_ptr(), 0, 100, None, 0, None) == L.AE_ERR_INVALID_ARG
     assert b"scratch" in lib.ae_last_error_message()
     assert lib.ae_points8_read(bank.handle, 0, None, 0, None, 0, 0, None) == L.AE_OK
 
@@ -343,7 +343,7 @@ def test_strides_of_gigabytes(A):
     bank.write(p.cuda())
     pv = U.values(n64(p))
     step = 9_000_000
-    for m in (3, 20):
+    for m in (3, 20, 70):
         room = torch.zeros((m - 1) * step + n, dtype=torch.bfloat16, device="cuda")
         dc = vectors(m, n, 2).bfloat16()
         far = room.as_strided((m, n), (step, 1))
@@ -401,7 +401,7 @@ def test_rows_behind_the_last_point_do_not_count(A):
     p = vectors(20, 100, 1)
     bank.write(p.cuda(), first=16)
     pv = U.values(n64(p))
-    for m in (2, 30):
+    for m in (2, 30, 70):
         room = torch.full((m + 2, 120), float("nan"), device="cuda")
         x = vectors(m, 100, 2)
         room[1:-1, 8:108] = x.cuda()
