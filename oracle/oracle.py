@@ -453,10 +453,13 @@ def direct_svd_epsil(mat, epsil, step, max_rank, rng=None):
 
 
 def svd_full(mat):
-    """svd_f32, graphlaplace.rs:296-344: gesdd JobSvd::Some -> s, u."""
+    """svd_f32, graphlaplace.rs:296-344: gesdd JobSvd::Some -> s, u.
+
+    Decomposed in 64 bits and rounded once: in f32 the vectors of two singular values 2e-5 apart turn by 1e-7 / 2e-5 and its growth over the
+    steps of the reduction, as much as the host's LAPACK kernels decide (5e-3 on one processor, 1e-2 on another, the same matrix)."""
     import scipy.linalg as sla
-    u, s, _ = sla.svd(mat, full_matrices=False, lapack_driver="gesdd", check_finite=False)
-    return s, u
+    u, s, _ = sla.svd(mat.astype(np.float64), full_matrices=False, lapack_driver="gesdd", check_finite=False)
+    return s.astype(mat.dtype), u.astype(mat.dtype)
 
 
 def estimate_first_singular_value(mat):
