@@ -271,14 +271,14 @@ __global__ void __launch_bounds__(256, 2) grad_tile_kernel(GradArgs a) {
 // dc of bf16, which the matrix cores take as it is.  16 FR rows x 128 coordinates; two waves share the coordinates, two the points of a step.  A lane
 // takes 4 coordinates of 8 points, one dword a point: put together by coordinate they are what the matrix cores want of it, with coordinates 4 apart
 // in a fragment, so the codes are widened in the registers they are used from, and each wave reads all rows of dc: LDS moves 48 KB for
-// 128 x 128 x 64 where the kernel above moves 112 (300 x 60 000 x 784: 49 us against 52, 4096 x 32 768 x 1024: 256 against 303, 1075 TF of the 1413 that a
+// 128 x 128 x 64 where the kernel above moves 112 (300 x 60 000 x 784: 47 us against 52, 4096 x 32 768 x 1024: 256 against 303, 1075 TF of the 1413 that a
 // large bf16 product of the library reaches).  dc and the codes come by copies to LDS three deep; the codes are read two steps ahead and widened under
 // the products, whose waits for one another and for the barrier of a step are what bounds it: the matrix cores are busy for 45 % of the time.
 constexpr int kTurnStage = kStep * 128;   // codes of a step
 template <int FR> constexpr int turn_lds() { return 3 * (16 * FR * kStep * 2 + kTurnStage + 1024); }   // 51 or 75 KB for 64 or 128 rows
 
 template <int FR>
-__global__ void __launch_bounds__(256, FR == 8 ? 2 : FR == 4 ? 3 : 4) grad_turn_kernel(GradArgs a) {
+__global__ void __launch_bounds__(256, 2) grad_turn_kernel(GradArgs a) {
     constexpr int STAGE = 16 * FR * kStep * 2, CODES = 3 * STAGE, SCALES = CODES + 3 * kTurnStage, COPIES_DC = FR / 2, COPIES = COPIES_DC + 3;
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     uint32_t slice, ti, tk;
@@ -478,16 +478,16 @@ GradPlan grad_plan(uint64_t m, uint64_t n, uint64_t dim, uint32_t dctype) {
     GradPlan best{};
     const uint64_t steps = std::max<uint64_t>((n + kStep - 1) / kStep, 1), tiles_k = (dim + kBlock - 1) / kBlock, ldp = (dim + 3) / 4 * 4;
     const uint64_t most = 0x3FFF0000ull / points8_row_bytes(dim) / kStep, least_slices = (steps + most - 1) / most;   // a slice's codes: less than 1 GiB
-    // What a choice costs, in us: a workgroup's beginning and end; its steps, with so many workgroups on a CU (measured at 300 x 60 000 x 784 in 7, 14 and 22
-    // slices of 64 rows and 12 and 24 of 128; more rows of f32, more workgroups of f16 and f32 do not fit); the slices' sums, written and read again at 5
-    // TB/s; the launch that joins them.  300 x 60 000 x 784 of bf16 takes 49 us as chosen, 49 to 60 with the other choices; 1024 rows 107 against 126 to
-    // 181; 1000 x 1000 x 1000 in one slice 12.6 against 16 to 21 in several.
+    // What a choice costs, in us: a workgroup's beginning and end; its steps, with so many workgroups on a CU (measured at 300 x 60 000 x 784, between operands
+    // in cache and operands from memory; more workgroups do not fit or do not pay); the slices' sums, written and read again at 5 TB/s; the launch that
+    // joins them.  bf16, from memory: 300 x 60 000 x 784 56 us with 128 rows and two workgroups on a CU, 58 to 65 otherwise; 64 rows of it 22.4 with 64
+    // and one, 24 to 27 otherwise; 1000 x 1000 x 1000 in one slice 12.6 against 16 to 21 in several.
     struct Choice { uint32_t fr, wgs; float step; };
-    static constexpr Choice bf16[] = {{1, 1, 0.41f}, {1, 2, 0.57f}, {1, 3, 0.84f}, {2, 1, 0.51f}, {2, 2, 0.82f}};
+    static constexpr Choice bf16[] = {{1, 1, 0.43f}, {1, 2, 0.66f}, {2, 1, 0.55f}, {2, 2, 0.86f}};
     static constexpr Choice f16[] = {{1, 1, 0.84f}, {1, 2, 1.1f}, {2, 1, 1.25f}, {2, 2, 1.76f}};
     static constexpr Choice f32[] = {{1, 1, 1.07f}, {1, 2, 1.46f}};
     const Choice* const choices = dctype == AE_TYPE_BF16 ? bf16 : dctype == AE_TYPE_F16 ? f16 : f32;
-    const int count = dctype == AE_TYPE_BF16 ? 5 : dctype == AE_TYPE_F16 ? 4 : 2;
+    const int count = dctype == AE_TYPE_F32 ? 2 : 4;
     double least = 0.;
     for (int q = 0; q < count; q++) {
         const Choice& c = choices[q];
@@ -495,7 +495,7 @@ GradPlan grad_plan(uint64_t m, uint64_t n, uint64_t dim, uint32_t dctype) {
         for (const uint64_t want : {(uint64_t)1, slots / tiles}) {
             const uint64_t slices = std::max<uint64_t>({1, least_slices, std::min(want, (steps + 3) / 4)}), per = (steps + slices - 1) / slices, used = (steps + per - 1) / per;
             const double rounds = (double)((tiles * used + slots - 1) / slots);
-            const double cost = rounds * ((c.fr == 1 ? 2 : 6) + per * c.step) + (used > 1 ? 4. + used * (0.005 + m * ldp * 8 / 5.1e6) : 0.);
+            const double cost = rounds * ((c.fr == 1 ? 2 : 5) + per * c.step) + (used > 1 ? 4. + used * (0.005 + m * ldp * 8 / 5.1e6) : 0.);
             if (best.fr && cost >= least) continue;
             least = cost;
             best = GradPlan{c.fr, tiles_m, tiles_k, used, per * kStep, ldp, used > 1 ? used * m * ldp * 4 : 0};
