@@ -334,14 +334,16 @@ __global__ void __launch_bounds__(64) teacher_join_kernel(const typename Elem<TY
     const uint32_t lane = threadIdx.x;
     const float w = weight ? weight[r] : 1.f;
     float m = -INFINITY, lnsum = 0.f, one = 0.f;
+    // (the slices' sums are on their way while the list is taken)
+    const float c = kLog2e / temperature;
+    Running run;
+    if (w != 0.f)
+        for (uint32_t q = lane; q < slices; q += 64) run.join(part[2 * (r * slices + q)], part[2 * (r * slices + q) + 1], c);
     if (w != 0.f) {
         const ListLds l(lds, list.k);
         double plogp;
         const double p_sum = take_list(list, r, cols, temperature, l, true, plogp);
         for (uint32_t j = lane; j < list.k; j += 64) l.logit[j] = l.col[j] == 0xFFFFFFFFu ? 0.f : (float)logits[r * ld + l.col[j]];
-        const float c = kLog2e / temperature;
-        Running run;
-        for (uint32_t q = lane; q < slices; q += 64) run.join(part[2 * (r * slices + q)], part[2 * (r * slices + q) + 1], c);
 #pragma unroll
         for (int o = 32; o; o >>= 1) {
             const float m2 = __shfl_xor(run.m, o), s2 = __shfl_xor(run.s, o);

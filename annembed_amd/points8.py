@@ -34,28 +34,27 @@ def _rows(t, what, device, shape=None):
     """pointer, type and row stride of a 2-D tensor whose rows are contiguous"""
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise _bad("%s has to be a 2-D tensor" % what)
-    if t.dtype not in _TYPES:
+    kind, (rows, cols), (ld, inner) = _TYPES.get(t.dtype), t.shape, t.stride()
+    if kind is None:
         raise _bad("%s is %s: float32, bfloat16 and float16 are taken" % (what, t.dtype))
     if t.device != device:
         raise _bad("%s is on %s, not on %s" % (what, t.device, device))
-    if shape is not None and tuple(t.shape) != shape:
-        raise _bad("%s has shape %s, not %s" % (what, tuple(t.shape), shape))
-    rows, cols = t.shape
-    ld, inner = t.stride()
-    if cols > 1 and inner != 1:
+    if shape is not None and (rows, cols) != shape:
+        raise _bad("%s has shape %s, not %s" % (what, (rows, cols), shape))
+    if inner != 1 and cols > 1:
         raise _bad("%s: the elements of a row have to be next to each other (stride %d)" % (what, inner))
-    if rows <= 1:
-        ld = max(ld, cols)
-    elif ld < cols:
-        raise _bad("%s: rows that overlap (stride %d of %d elements)" % (what, ld, cols))
-    return t.data_ptr(), _TYPES[t.dtype], ld
+    if ld < cols:
+        if rows > 1:
+            raise _bad("%s: rows that overlap (stride %d of %d elements)" % (what, ld, cols))
+        ld = cols
+    return t.data_ptr(), kind, ld
 
 
 def _vector(t, what, device, n, dtypes):
     """pointer of a contiguous 1-D tensor of n elements, or None"""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.shape[0] != n or t.dtype not in dtypes:
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.shape != (n,):
         raise _bad("%s has to be a 1-D tensor of %d elements of %s" % (what, n, " or ".join(str(d) for d in dtypes)))
     if t.device != device:
         raise _bad("%s is on %s, not on %s" % (what, t.device, device))
@@ -69,16 +68,19 @@ _INDEX = (torch.int32, torch.uint32)
 
 # the current stream of a device as an integer: the public torch.cuda.current_stream() builds an object first, for 2.5 us a call
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device   # (the public one looks whether CUDA is initialised first)
 
 
 def _call(device, fn, *args):
     """the library call on torch's current stream of `device`, which has to be the current device while it runs"""
-    f = getattr(L.load(), fn)
-    if torch.cuda.current_device() == device.index:
-        check(f(*args, _stream(device.index)))
+    f, index = getattr(L.load(), fn), device.index
+    if _device() == index:
+        rc = f(*args, _stream(index))
     else:
         with torch.cuda.device(device):
-            check(f(*args, _stream(device.index)))
+            rc = f(*args, _stream(index))
+    if rc != L.AE_OK:   # (none of these calls leaves a warning)
+        check(rc)
 
 
 @functools.lru_cache(maxsize=1024)
