@@ -16,6 +16,10 @@ constexpr int kTrips = 4;      // blocks a group has in flight: 64 to 128 bytes 
 // the two or three launches otherwise, 5000 of 784 7.3 against 11.1; 8191 of 128 10.1 against 8.0, 8000 of 1500 18.4 against 16.0.
 constexpr uint32_t kScan = 6000;
 
+// Up to this many blocks a group of lanes takes one, so that few rows spread over more workgroups (4096 scattered rows of 128: 6.9 against 20 us with
+// kTrips; beyond, each workgroup's look at all slots costs more than that: 4096 rows of 4096 18.5 against 16.2).
+constexpr uint64_t kSpread = 65536;
+
 struct Blocks {   // the call's blocks
     uint64_t units, n;
     uint32_t nb;
@@ -130,21 +134,21 @@ __global__ void __launch_bounds__(256) points8_write_kernel(const typename Elem<
     }
 }
 
-template <int TYPE, bool SLOTS>
+template <int TYPE, bool SLOTS, int TRIPS>
 __global__ void __launch_bounds__(256) points8_read_kernel(const uint8_t* __restrict__ codes, uint64_t row_bytes, const uint8_t* __restrict__ scales, uint64_t scale_stride,
                                                            uint64_t capacity, uint64_t first, const uint32_t* __restrict__ slots, Blocks bl,
                                                            typename Elem<TYPE>::T* __restrict__ x, uint64_t ldx, uint64_t dim) {
-    const uint64_t u0 = blockIdx.x * (uint64_t)(kGroups * kTrips);
+    const uint64_t u0 = blockIdx.x * (uint64_t)(kGroups * TRIPS);
     const Cursor cur(u0, bl.nb);
     const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
-    uint2 c[kTrips];
-    uint32_t byte[kTrips];
-    uint64_t row[kTrips];
-    uint32_t b[kTrips];
-    int count[kTrips];
-    bool bad[kTrips];
+    uint2 c[TRIPS];
+    uint32_t byte[TRIPS];
+    uint64_t row[TRIPS];
+    uint32_t b[TRIPS];
+    int count[TRIPS];
+    bool bad[TRIPS];
 #pragma unroll
-    for (int t = 0; t < kTrips; t++) {
+    for (int t = 0; t < TRIPS; t++) {
         const uint32_t off = t * kGroups + group;
         cur.at(off, bl.nb, row[t], b[t]);
         const uint64_t k = b[t] * (uint64_t)kBlock + lane * 8;
@@ -165,7 +169,7 @@ __global__ void __launch_bounds__(256) points8_read_kernel(const uint8_t* __rest
         }
     }
 #pragma unroll
-    for (int t = 0; t < kTrips; t++) {
+    for (int t = 0; t < TRIPS; t++) {
         float v[8];
         decode8(c[t], byte[t], v);
         if (SLOTS && bad[t]) {
@@ -190,32 +194,34 @@ unsigned trips_grid(const Blocks& bl, int trips) {
     return (unsigned)g;
 }
 
-template <int SLOTS, int TRIPS = kTrips>
+template <int SLOTS>
 void launch_write(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint64_t first, const uint32_t* slots, uint32_t* owner, uint64_t capacity,
                   uint8_t* codes, uint8_t* scales, uint64_t scale_stride, hipStream_t s) {
     const Blocks bl = blocks_of(n, dim);
-    const unsigned grid = trips_grid(bl, TRIPS);
     by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         const auto* x = static_cast<const typename Elem<TYPE>::T*>(d_x);
-        hipLaunchKernelGGL((points8_write_kernel<TYPE, SLOTS, TRIPS>), dim3(grid), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales,
-                           scale_stride);
+        auto go = [&](auto kernel, int trips) {
+            hipLaunchKernelGGL(kernel, dim3(trips_grid(bl, trips)), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales, scale_stride);
+        };
+        if (bl.units <= kSpread) go(points8_write_kernel<TYPE, SLOTS, 1>, 1);
+        else go(points8_write_kernel<TYPE, SLOTS, kTrips>, kTrips);
     });
     check_launch("points8_write");
 }
 
 void read_rows(const ae_points8* p, uint64_t first, const uint32_t* slots, uint64_t n, void* d_x, uint32_t type, uint64_t ldx, hipStream_t s) {
     const Blocks bl = blocks_of(n, p->dim);
-    const unsigned grid = trips_grid(bl, kTrips);
     by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         auto* x = static_cast<typename Elem<TYPE>::T*>(d_x);
-        auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, (const uint8_t*)p->codes.p, p->row_bytes, (const uint8_t*)p->scales.p, p->scale_stride, p->capacity, first,
+        auto go = [&](auto kernel, int trips) {
+            hipLaunchKernelGGL(kernel, dim3(trips_grid(bl, trips)), dim3(256), 0, s, (const uint8_t*)p->codes.p, p->row_bytes, (const uint8_t*)p->scales.p, p->scale_stride, p->capacity, first,
                                slots, bl, x, ldx, p->dim);
         };
-        if (slots) go(points8_read_kernel<TYPE, true>);
-        else go(points8_read_kernel<TYPE, false>);
+        const bool spread = bl.units <= kSpread;
+        if (slots) spread ? go(points8_read_kernel<TYPE, true, 1>, 1) : go(points8_read_kernel<TYPE, true, kTrips>, kTrips);
+        else spread ? go(points8_read_kernel<TYPE, false, 1>, 1) : go(points8_read_kernel<TYPE, false, kTrips>, kTrips);
     });
     check_launch("points8_read");
 }
@@ -301,10 +307,7 @@ int32_t ae_points8_write(ae_points8* p, const void* d_x, uint32_t type, uint64_t
         // The last row of a repeated slot is held.  Few rows: every workgroup looks at the slots behind its own, one launch.  More: the rows claim
         // their slots first and give them back as they are written, or, rows of several blocks, in a launch of their own.
         if (n <= kScan) {
-            // one block a group of lanes spreads few rows over more workgroups (4096 rows of 128: 6.9 against 20 us with four), but each of them looks
-            // at all slots (4096 rows of 4096: 18.5 against 16.2)
-            if (n * p->blocks <= 65536) launch_write<1, 1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
-            else launch_write<1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
+            launch_write<1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
             return;
         }
         const unsigned grid = blocks_for(n, 256);
