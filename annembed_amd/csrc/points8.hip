@@ -16,9 +16,11 @@ constexpr int kTrips = 4;      // blocks a group has in flight: 64 to 128 bytes 
 // the two or three launches otherwise, 5000 of 784 7.3 against 11.1; 8191 of 128 10.1 against 8.0, 8000 of 1500 18.4 against 16.0.
 constexpr uint32_t kScan = 6000;
 
-// Up to this many blocks a group of lanes takes one, so that few rows spread over more workgroups (4096 scattered rows of 128: 6.9 against 20 us with
-// kTrips; beyond, each workgroup's look at all slots costs more than that: 4096 rows of 4096 18.5 against 16.2).
-constexpr uint64_t kSpread = 65536;
+// Whether a group of lanes takes one block instead of kTrips: fewer loads in flight, more waves.  f32 (32 bytes of loads a lane and block) always, 16 bits up
+// to a million blocks (write 60 000 x 784 of bf16 26 against 30 us, 262 144 x 1024 145 against 148, but read 200 000 x 784 by ids 139 against 116; f32 read
+// 200 000 x 784 137 against 200, write 8191 x 128 scattered 6.8 against 8.1).  Workgroups that look at all slots of the call: while they are few (4096
+// rows of 128 6.9 against 20 us, 4096 rows of 4096 18.5 against 16.2).
+bool spread(uint64_t units, uint32_t type, bool look) { return units <= (look ? 65536 : type == AE_TYPE_F32 ? 1 << 27 : 1 << 20); }
 
 struct Blocks {   // the call's blocks
     uint64_t units, n;
@@ -204,7 +206,7 @@ void launch_write(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint
         auto go = [&](auto kernel, int trips) {
             hipLaunchKernelGGL(kernel, dim3(trips_grid(bl, trips)), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales, scale_stride);
         };
-        if (bl.units <= kSpread) go(points8_write_kernel<TYPE, SLOTS, 1>, 1);
+        if (spread(bl.units, type, SLOTS == 1)) go(points8_write_kernel<TYPE, SLOTS, 1>, 1);
         else go(points8_write_kernel<TYPE, SLOTS, kTrips>, kTrips);
     });
     check_launch("points8_write");
@@ -219,9 +221,9 @@ void read_rows(const ae_points8* p, uint64_t first, const uint32_t* slots, uint6
             hipLaunchKernelGGL(kernel, dim3(trips_grid(bl, trips)), dim3(256), 0, s, (const uint8_t*)p->codes.p, p->row_bytes, (const uint8_t*)p->scales.p, p->scale_stride, p->capacity, first,
                                slots, bl, x, ldx, p->dim);
         };
-        const bool spread = bl.units <= kSpread;
-        if (slots) spread ? go(points8_read_kernel<TYPE, true, 1>, 1) : go(points8_read_kernel<TYPE, true, kTrips>, kTrips);
-        else spread ? go(points8_read_kernel<TYPE, false, 1>, 1) : go(points8_read_kernel<TYPE, false, kTrips>, kTrips);
+        const bool one = spread(bl.units, type, false);
+        if (slots) one ? go(points8_read_kernel<TYPE, true, 1>, 1) : go(points8_read_kernel<TYPE, true, kTrips>, kTrips);
+        else one ? go(points8_read_kernel<TYPE, false, 1>, 1) : go(points8_read_kernel<TYPE, false, kTrips>, kTrips);
     });
     check_launch("points8_read");
 }
