@@ -12,8 +12,8 @@ namespace {
 
 constexpr int kGroups = 16;    // blocks per workgroup and trip
 constexpr int kTrips = 4;      // blocks a group has in flight: 64 to 128 bytes of loads per lane
-// Up to this many slots a workgroup looks for later occurrences of its rows' slots itself, in one launch: 4096 rows of 128 take 6.9 us against 8.0 of
-// the two or three launches otherwise, 5000 of 784 7.3 against 11.1; 8191 of 128 10.1 against 8.0, 8000 of 1500 18.4 against 16.0.
+// Up to this many slots a workgroup looks for later occurrences of its rows' slots itself, in one launch, rows of one block up to 4096: 4096 rows of 128 take 6.9
+// us against 7.1 of the two launches otherwise, 8191 of 128 10.1 against 7.1; 5000 of 784 7.3 against 11.1 of three, 8000 of 1500 18.4 against 16.0.
 constexpr uint32_t kScan = 6000;
 
 // Whether a group of lanes takes one block instead of kTrips: fewer loads in flight, more waves.  f32 (32 bytes of loads a lane and block) always, 16 bits up
@@ -308,7 +308,7 @@ int32_t ae_points8_write(ae_points8* p, const void* d_x, uint32_t type, uint64_t
         if (n > 0x7FFFFFFFull) fail(AE_ERR_INVALID_ARG, "ae_points8_write: %llu slots are more than one call takes", (unsigned long long)n);
         // The last row of a repeated slot is held.  Few rows: every workgroup looks at the slots behind its own, one launch.  More: the rows claim
         // their slots first and give them back as they are written, or, rows of several blocks, in a launch of their own.
-        if (n <= kScan) {
+        if (n <= (p->blocks == 1 ? 4096 : kScan)) {
             launch_write<1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
             return;
         }
