@@ -316,6 +316,96 @@ product_tile_kernel(ProductArgs a) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the copies of nothing have ended before the LDS is given back
 }
 
+// Few tiles of long rows: a workgroup owns 64 x 64, its four waves take every fourth block of 128 coordinates of it and their sums are added last, in order.
+// Operands go from memory to the lanes that multiply them (32 bytes of 16 rows an access: the caches take 64 lanes one by one, which a chip with
+// little to do has time for), the next block's while this one's are multiplied.  Rows of a lane as above: four neighbours, their scales a dword.
+template <int TYPE>
+__global__ void __launch_bounds__(256, 2) product_deep_kernel(ProductArgs a) {
+    constexpr bool EXACT = TYPE == AE_TYPE_F32;
+    using T = typename Elem<TYPE>::T;
+    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
+    const uint32_t tn = blockIdx.x / a.tiles_m, tm = blockIdx.x - tn * a.tiles_m;
+    const uint64_t i0 = (uint64_t)tm * 64, j0 = (uint64_t)tn * 64;
+    const uint32_t mi = (uint32_t)min((uint64_t)64, a.x.rows - i0), nj = (uint32_t)min((uint64_t)64, a.p.rows - j0), stride = (uint32_t)a.x.row_bytes;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
+    __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x.codes + i0 * stride), (short)0, (int)(mi * stride), 0x00027000);
+    __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.codes + j0 * stride), (short)0, (int)(nj * stride), 0x00027000);
+    const uint8_t *sx = a.x.scales + i0 + (lane & 15) * 4, *sp = a.p.scales + j0 + (lane & 15) * 4;
+    const uint32_t row_at = (lane & 15) * 4 * stride + g * 32;
+    struct Block { u32x4 x[4][2], p[4][2]; uint32_t bx, bp; } now, next;
+    auto load = [&](uint32_t kb, Block& b) {   // (past the last block or a row's last byte: zeros)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t at = kb * kBlock + g * 32 + h * 16 < stride ? 0u : 0x40000000u;
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                const int off = (int)((row_at + f * stride + kb * kBlock + h * 16) | at);
+                b.x[f][h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 0, 0));
+                b.p[f][h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, off, 0, 0));
+            }
+        }
+        const uint64_t last = min(kb, a.blocks - 1);
+        __builtin_memcpy(&b.bx, sx + last * a.x.scale_stride, 4);
+        __builtin_memcpy(&b.bp, sp + last * a.p.scale_stride, 4);
+    };
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    load(wave, now);
+    for (uint32_t kb = wave; kb < a.blocks; kb += 4) {
+        load(kb + 4, next);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                bf16x8 wp[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) wp[j] = widen8(now.p[j][e >> 1][(e & 1) * 2], now.p[j][e >> 1][(e & 1) * 2 + 1], now.bp >> (j * 8) & 255u);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const bf16x8 wx = widen8(now.x[i][e >> 1][(e & 1) * 2], now.x[i][e >> 1][(e & 1) * 2 + 1], now.bx >> (i * 8) & 255u);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp[j], wx, acc[i][j], 0, 0, 0);
+                }
+            }
+        } else {
+#define AE_ONE(I, J) acc[I][J] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(now.p[J][0], now.p[J][1]), join(now.x[I][0], now.x[I][1]), acc[I][J], 0, 0, J, (int)now.bp, I, (int)now.bx);
+#define AE_ROW(I) AE_ONE(I, 0) AE_ONE(I, 1) AE_ONE(I, 2) AE_ONE(I, 3)
+            AE_ROW(0) AE_ROW(1) AE_ROW(2) AE_ROW(3)
+#undef AE_ROW
+#undef AE_ONE
+        }
+        now = next;
+    }
+    f32x4* part = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) part[(wave * 16 + i * 4 + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    // wave i adds the rows i of the lanes: columns 16 g + 4 e + j
+    f32x4 sum[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        sum[j] = part[(wave * 4 + j) * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < 4; w++) sum[j] += part[(w * 16 + wave * 4 + j) * 64 + lane];
+    }
+    const uint32_t row = (lane & 15) * 4 + wave, col = g * 16;
+    if (row >= mi) return;
+    T* c = static_cast<T*>(a.c) + (i0 + row) * a.ldc + j0 + col;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; q++) v[q] = sum[q & 3][h * 2 + (q >> 2)];
+        const int count = (int)nj - (int)col - h * 8;
+        if (count > 0) store8<TYPE>(c + h * 8, min(count, 8), v);
+    }
+}
+
 template <int BM, int BN, int WM>
 void launch_tiles(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t ctype, uint64_t ldc, hipStream_t s) {
     const uint64_t tiles_m = (x.rows + BM - 1) / BM, tiles_n = (p.rows + BN - 1) / BN, tiles = tiles_m * tiles_n;
@@ -335,6 +425,19 @@ void launch_tiles(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint3
 // little (4096 x 4096 x 1024 to bf16: 21.6 against 23.9 us with 128 x 128, 8192^3: 418 against 585; 1024 x 10 000 x 784, 160 tiles: 20.5
 // against 19.4; 300 x 60 000 x 784, two rows of tiles for 300: 35.3 against 30.9).
 void product(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t ctype, uint64_t ldc, hipStream_t s) {
+    // Workgroups of 64 x 64 that split the coordinates, while each has a CU of its own, or nearly (170 x 258 x 1986 to bf16 8.1 against 11.8 us with 128 x 128 tiles, to f32
+    // 9.7 against 19.9; 1000 x 1000 x 1000, 256 of them, 6.5 against 8.1 and 8.3 against 13.4; 120 x 9069 x 1609, 284, 14.4 against 13.6 and 16.4 against 21.3;
+    // 512 x 4096 x 512, 512, 7.8 against 6.4 and 10.3 against 9.6).
+    const uint64_t deep_m = (x.rows + 63) / 64, deep_n = (p.rows + 63) / 64;
+    if (deep_m * deep_n <= (ctype == AE_TYPE_F32 ? 384 : 256)) {
+        const ProductArgs a{x, p, points8_blocks(dim), d_c, ldc, (uint32_t)deep_m, (uint32_t)deep_n, 0};
+        by_type(ctype, [&](auto ty) {
+            constexpr int TYPE = decltype(ty)::value;
+            hipLaunchKernelGGL((product_deep_kernel<TYPE>), dim3((unsigned)(deep_m * deep_n)), dim3(256), 4 * 16 * 64 * 16, s, a);
+        });
+        check_launch("points8_product_deep");
+        return;
+    }
     const uint64_t tm = (x.rows + 255) / 256, tn = (p.rows + 255) / 256;
     if (tm * tn >= 256 && tm * 256 * 4 <= x.rows * 5 && tn * 256 * 4 <= p.rows * 5) launch_tiles<256, 256, 128>(x, p, dim, d_c, ctype, ldc, s);
     else launch_tiles<128, 128, 64>(x, p, dim, d_c, ctype, ldc, s);
