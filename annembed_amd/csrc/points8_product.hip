@@ -448,11 +448,15 @@ void product(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t c
 // launch.  SPLIT waves share the blocks of a group of points where there are few points.
 constexpr int kFew = 64;
 constexpr uint64_t few_lds_row(uint64_t dim) { return ((dim + kBlock - 1) / kBlock * kBlock) * 2 + 16; }   // (16 bytes more: neighbours start 4 banks apart)
-// From 17 rows on while the products are few: every workgroup's own quantising and the exact bf16 products cost more than a second launch then (32 x 2000 x 300
-// of f32: 7.8 against 11.3 us; 17 x 60 000 x 128: 8.6 against 10.3; 17 x 20 000 x 700: 14.6 against 13.7; 48 x 60 000 x 128: 17.0 against 11.7).
+// 16 points a wave leave half of the chip's waves without work below 32 768 points: four waves share them then
+uint64_t few_points(uint64_t n, uint64_t dim) { return n >= 32768 || points8_blocks(dim) < 4 ? 64 : 16; }
+// One launch while the quantising that every workgroup does for itself, and the exact products, cost less than a launch does (one row against 5000 x 4000
+// 7.0 against 15.7 us, 16 against 3000 x 1400 9.1 against 10.3, but against 30 000 x 1400 33 against 18; 17 against 2000 x 300 6.1 against 8.2, 32
+// against 30 000 x 128 7.0 against 8.5, against 20 000 x 300 9.4 against 8.3; 48 against 20 000 x 28 9.1 against 8.2).
 bool few_rows(uint64_t m, uint64_t n, uint64_t dim) {
     if (m > kFew || m * few_lds_row(dim) > 48 * 1024 || n >= 1ull << 30) return false;   // (64 points, 256 threads: fewer than 2^32)
-    return m <= 16 || (m * n <= 1 << 20 && m * n * dim <= 200000000);
+    const uint64_t tiles = m <= 16 ? 1 : m <= 32 ? 2 : 4, quantised = (n + few_points(n, dim) - 1) / few_points(n, dim) * m * dim;
+    return m <= 16 ? quantised <= 10000000 : tiles * 16 * n <= 1 << 20 && m * dim <= 10000 && quantised <= 2000000;
 }
 
 template <int XTYPE, int SPLIT, int TILES>   // TILES of 16 rows
@@ -553,8 +557,7 @@ void product_few(const void* d_x, uint32_t xtype, uint64_t m, uint64_t ldx, uint
             hipLaunchKernelGGL(kernel, dim3((unsigned)((p.rows + points - 1) / points)), dim3(256), bytes, s, static_cast<const typename Elem<TYPE>::T*>(d_x), (uint32_t)m, ldx,
                                (uint32_t)dim, p, d_c, ctype, ldc);
         };
-        // 16 points a wave leave half of the chip's waves without work below 32 768 points: four waves share them then
-        const bool whole = p.rows >= 32768 || points8_blocks(dim) < 4;
+        const bool whole = few_points(p.rows, dim) == 64;
         if (tiles == 1) whole ? go(product_few_kernel<TYPE, 1, 1>, 64) : go(product_few_kernel<TYPE, 4, 1>, 16);
         else if (tiles == 2) whole ? go(product_few_kernel<TYPE, 1, 2>, 64) : go(product_few_kernel<TYPE, 4, 2>, 16);
         else whole ? go(product_few_kernel<TYPE, 1, 4>, 64) : go(product_few_kernel<TYPE, 4, 4>, 16);

@@ -124,7 +124,7 @@ def product_bound(x, p, terms, want, dtype, eights=False):
     return (terms * 2.0 ** -23 + eights * 7 * 2.0 ** -13) * (np.abs(x) @ np.abs(p)) + f.eps / 2 * np.maximum(np.abs(want), f.smallest_normal)
 
 
-@pytest.mark.parametrize("m,n,dim", [(1, 1, 1), (1, 3, 28), (1, 1000, 784), (17, 33000, 28), (31, 700, 600), (50, 3000, 200), (64, 16384, 10), (700, 4100, 130), (129, 33000, 100), (4100, 4200, 140), (2500, 2600, 28), (65, 16300, 520), (2, 129, 128), (5, 64, 130), (16, 500, 784), (17, 257, 100), (33, 31, 1000), (64, 2000, 16), (127, 128, 129),
+@pytest.mark.parametrize("m,n,dim", [(1, 1, 1), (1, 3, 28), (1, 1000, 784), (17, 32768, 28), (20, 1500, 500), (31, 700, 600), (9, 3000, 1500), (50, 3000, 200), (64, 16384, 10), (700, 4100, 130), (129, 33000, 100), (4100, 4200, 140), (2500, 2600, 28), (65, 16300, 520), (2, 129, 128), (5, 64, 130), (16, 500, 784), (17, 257, 100), (33, 31, 1000), (64, 2000, 16), (127, 128, 129),
                                      (128, 128, 256), (129, 385, 640), (200, 1111, 784), (300, 700, 2000), (513, 1025, 64), (1, 40, 9000)])
 def test_product(A, m, n, dim):
     bank = A.Points8(n + 5, dim)
