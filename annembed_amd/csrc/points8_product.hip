@@ -560,7 +560,7 @@ void product_few(const void* d_x, uint32_t xtype, uint64_t m, uint64_t ldx, uint
         const bool whole = few_points(p.rows, dim) == 64;
         if (tiles == 1) whole ? go(product_few_kernel<TYPE, 1, 1>, 64) : go(product_few_kernel<TYPE, 4, 1>, 16);
         else if (tiles == 2) whole ? go(product_few_kernel<TYPE, 1, 2>, 64) : go(product_few_kernel<TYPE, 4, 2>, 16);
-        else whole ? go(product_few_kernel<TYPE, 1, 4>, 64) : go(product_few_kernel<TYPE, 4, 4>, 16);
+        else go(product_few_kernel<TYPE, 1, 4>, 64);   // (33 rows or more have at most 303 coordinates)
     });
     check_launch("points8_product_few");
 }

@@ -460,9 +460,13 @@ void launch_rows(const Call& a) {
         else if (pieces <= 512) go(teacher_row_kernel<TYPE, 256, 2, LOSS>, 256);
         else if (pieces <= 1024) go(teacher_row_kernel<TYPE, 256, 4, LOSS>, 256);
         else if (pieces <= 2048) go(teacher_row_kernel<TYPE, 256, 8, LOSS>, 256);
-        else if (pieces <= 4096) go(teacher_row_kernel<TYPE, 512, 8, LOSS>, 512);
-        else if (pieces <= 8192) go(teacher_row_kernel<TYPE, 1024, 8, LOSS>, 1024);
-        else if constexpr (TYPE == AE_TYPE_F32) go(teacher_row_kernel<TYPE, 1024, 16, LOSS>, 1024);
+        else if constexpr (LOSS || TYPE == AE_TYPE_F32) {   // (the gradient alone has slices from kLong columns on)
+            if (pieces <= 4096) go(teacher_row_kernel<TYPE, 512, 8, LOSS>, 512);
+            else if constexpr (LOSS) {
+                if (pieces <= 8192) go(teacher_row_kernel<TYPE, 1024, 8, true>, 1024);
+                else if constexpr (TYPE == AE_TYPE_F32) go(teacher_row_kernel<TYPE, 1024, 16, true>, 1024);
+            }
+        }
     });
     check_launch("teacher_row");
 }
