@@ -69,7 +69,6 @@ inline void by_type(uint32_t type, F&& f) {
 
 using f32x2 = __attribute__((ext_vector_type(2))) float;
 using f32x4 = __attribute__((ext_vector_type(4))) float;
-using i32x8 = __attribute__((ext_vector_type(8))) int;
 using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;

@@ -1,13 +1,10 @@
-// points8_product.hip -- rows times the points held in 8 bits: c[i][j] = <x_i, p_j> on the scaled 8-bit matrix cores.
+// points8_product.hip -- rows times the points held in 8 bits: c[i][j] = <x_i, p_j>, exact products with f32 sums.
 //
-// v_mfma_scale_f32_16x16x128_f8f6f4 takes 16 + 16 rows of 128 e4m3 codes with a power-of-two scale per row and 32 coordinates: a block with its
-// own scale byte, so the scales cost no arithmetic at all.  Which of the 128 coordinates a lane holds does not matter as long as both
-// operands agree.  (The 32 x 32 x 64 form does the same work for more power: 3.5 against 4.0 PFLOP/s on random codes, nothing but products.)
-//
-// The 8-bit cores add eight products of consecutive codes at a time, cut 13 bits below the largest of the eight (measured on this chip:
-// 2^12 + 2^-1 is kept, 2^12 + 2^-2 is 2^12).  That is at most 7 * 2^-13 of the sum of the products' magnitudes, 1e-5 of it in the
-// root mean square over encoder-like rows: below a 16-bit result's own rounding, not below an f32 result's.  So c of 16 bits takes the 8-bit
-// cores, and c of f32 takes the bf16 cores at half their rate: every value held is exact in bf16, the products too, the sums are f32.
+// Codes travel as 8 bits through memory and LDS and are widened, with their block's power of two, in the registers they are multiplied from: every
+// value held is exact in bf16, so are the products, and the bf16 matrix cores add them in f32.  The scaled 8-bit cores would do the products at twice
+// the rate, but they add eight of them at a time and cut 13 bits below the largest of the eight (measured on this chip: 2^12 + 2^-1 is kept,
+// 2^12 + 2^-2 is 2^12): where two large products cancel, the small ones beside them are lost.  Sums are held in 32 bits here, whatever the result's
+// type and however many rows there are.
 #include "points8.h"
 
 #include <algorithm>
@@ -16,9 +13,6 @@ using namespace ae;
 
 namespace {
 
-__device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b) {
-    return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
-}
 // the scale byte of row i of the FM (FN) that a lane holds, four of them in a dword
 __device__ __forceinline__ uint32_t byte_of(const uint32_t* dwords, int i) { return (dwords[i >> 2] >> ((i & 3) * 8)) & 255u; }
 
@@ -74,7 +68,7 @@ struct Walk {
 // BM x BN tiles of c, waves of WM x 64, a block of 128 coordinates per step, two stages of LDS in turn.
 //
 // Rows: fragment i of a wave's WM rows is rows i, i + FM, i + 2 FM ... of them (FM = WM / 16): the FM rows of a lane are neighbours, their
-// scale bytes one or two dwords, and the matrix cores pick the byte.  The same for the points, so a lane ends up with 16 consecutive
+// scale bytes one or two dwords.  The same for the points, so a lane ends up with 16 consecutive
 // columns of each of its rows and writes them itself.
 // LDS: fragment by fragment, a row's 128 codes as 8 chunks of 16 bytes, chunk c of LDS row r at place c ^ ((r >> 1) & 7).  The lanes of group g read
 // chunks g and g + 4: the 16 lanes that LDS serves at a time (0-3, 12-15 and 20-27 of a half wave, then the others) touch all 64 banks once.  (With chunks
@@ -89,8 +83,7 @@ __global__ void __launch_bounds__((BM / WM) * (BN / 64) * 64, (BM + BN) * kBlock
 product_tile_kernel(ProductArgs a) {
     constexpr int WN = 64, WAVES = (BM / WM) * (BN / WN), FM = WM / 16, FN = WN / 16;
     constexpr int STAGE = (BM + BN) * kBlock;
-    constexpr bool EXACT = TYPE == AE_TYPE_F32;
-    constexpr int STEPS = EXACT ? 2 * FM : FM;   // a step: FM-th part of the rows, the whole block or (f32) a half of it
+    constexpr int STEPS = 2 * FM;   // a step: FM-th part of the rows, a half of the block
     using T = typename Elem<TYPE>::T;
     constexpr int STORES = FM * (int)sizeof(T);
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
@@ -162,19 +155,13 @@ product_tile_kernel(ProductArgs a) {
 #pragma unroll
             for (int j = 0; j < FN; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     };
-    i32x8 fx[4], fp[FN];        // of f32 only the first halves
-    bf16x8 wp[FN][2];           // f32: the points' values of half a block
+    u32x4 fx[4], fp[FN];        // codes
+    bf16x8 wp[FN][2];           // the points' values of half a block
     const int r_x = wi + (lane & 15), r_p = BM + wj + (lane & 15), c0 = lane >> 4;
     uint32_t in_x = r_x * kBlock + ((c0 ^ ((r_x >> 1) & 7)) << 4), in_p = r_p * kBlock + ((c0 ^ ((r_p >> 1) & 7)) << 4);
     auto chunk_at = [&](uint32_t at) { return *reinterpret_cast<const u32x4*>(lds + at); };
-    auto read_x = [&](int s) {
-        if constexpr (EXACT) fx[s & 3] = join(chunk_at((in_x ^ (s / FM * 64)) + s % FM * 16 * kBlock), u32x4{0, 0, 0, 0});
-        else fx[s & 3] = join(chunk_at(in_x + s * 16 * kBlock), chunk_at((in_x ^ 64) + s * 16 * kBlock));
-    };
-    auto read_p = [&](int j, int h) {
-        if constexpr (EXACT) fp[j] = join(chunk_at((in_p ^ (h * 64)) + j * 16 * kBlock), u32x4{0, 0, 0, 0});
-        else fp[j] = join(chunk_at(in_p + j * 16 * kBlock), chunk_at((in_p ^ 64) + j * 16 * kBlock));
-    };
+    auto read_x = [&](int s) { fx[s & 3] = chunk_at((in_x ^ (s / FM * 64)) + s % FM * 16 * kBlock); };
+    auto read_p = [&](int j, int h) { fp[j] = chunk_at((in_p ^ (h * 64)) + j * 16 * kBlock); };
     auto block = [&](uint32_t stage, auto first) {
 #pragma unroll
         for (int q = 0; q < FM / 4; q++) bx[q] = nx[q];
@@ -196,37 +183,24 @@ product_tile_kernel(ProductArgs a) {
             }
             read_x((s + 2) % STEPS);
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (EXACT) {
-                const int h = s / FM, i = s % FM;
-                if (i == 0) {
+            const int h = s / FM, i = s % FM;
+            if (i == 0) {
 #pragma unroll
-                    for (int j = 0; j < FN; j++) {
+                for (int j = 0; j < FN; j++) {
 #pragma unroll
-                        for (int e = 0; e < 2; e++) wp[j][e] = widen8((uint32_t)fp[j][2 * e], (uint32_t)fp[j][2 * e + 1], byte_of(bp, j));
-                        if (h == 0) read_p(j, 1);
-                    }
+                    for (int e = 0; e < 2; e++) wp[j][e] = widen8(fp[j][2 * e], fp[j][2 * e + 1], byte_of(bp, j));
+                    if (h == 0) read_p(j, 1);
                 }
+            }
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const bf16x8 wx = widen8((uint32_t)fx[s & 3][2 * e], (uint32_t)fx[s & 3][2 * e + 1], byte_of(bx, i));
+            for (int e = 0; e < 2; e++) {
+                const bf16x8 wx = widen8(fx[s & 3][2 * e], fx[s & 3][2 * e + 1], byte_of(bx, i));
 #pragma unroll
-                    for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp[j][e], wx, acc[i][j], 0, 0, 0);
-                }
-                if (s == STEPS - 1) {
+                for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp[j][e], wx, acc[i][j], 0, 0, 0);
+            }
+            if (s == STEPS - 1) {
 #pragma unroll
-                    for (int j = 0; j < FN; j++) read_p(j, 0);
-                }
-            } else {
-#define AE_STEP(J, I)                                                                                                                             \
-    acc[s][J] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp[J], fx[s & 3], acc[s][J], 0, 0, J, (int)bp[0], I, (int)bx[s >> 2]);           \
-    if (s == STEPS - 1) read_p(J, 0);
-#define AE_STEPS(I) AE_STEP(0, I) AE_STEP(1, I) AE_STEP(2, I) AE_STEP(3, I)
-                if ((s & 3) == 0) { AE_STEPS(0) }
-                else if ((s & 3) == 1) { AE_STEPS(1) }
-                else if ((s & 3) == 2) { AE_STEPS(2) }
-                else { AE_STEPS(3) }
-#undef AE_STEPS
-#undef AE_STEP
+                for (int j = 0; j < FN; j++) read_p(j, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -321,7 +295,6 @@ product_tile_kernel(ProductArgs a) {
 // little to do has time for), the next block's while this one's are multiplied.  Rows of a lane as above: four neighbours, their scales a dword.
 template <int TYPE>
 __global__ void __launch_bounds__(256, 2) product_deep_kernel(ProductArgs a) {
-    constexpr bool EXACT = TYPE == AE_TYPE_F32;
     using T = typename Elem<TYPE>::T;
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const uint32_t tn = blockIdx.x / a.tiles_m, tm = blockIdx.x - tn * a.tiles_m;
@@ -357,25 +330,17 @@ __global__ void __launch_bounds__(256, 2) product_deep_kernel(ProductArgs a) {
     for (uint32_t kb = wave; kb < a.blocks; kb += 4) {
         load(kb + 4, next);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (EXACT) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                bf16x8 wp[4];
+        for (int e = 0; e < 4; e++) {
+            bf16x8 wp[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) wp[j] = widen8(now.p[j][e >> 1][(e & 1) * 2], now.p[j][e >> 1][(e & 1) * 2 + 1], now.bp >> (j * 8) & 255u);
+            for (int j = 0; j < 4; j++) wp[j] = widen8(now.p[j][e >> 1][(e & 1) * 2], now.p[j][e >> 1][(e & 1) * 2 + 1], now.bp >> (j * 8) & 255u);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const bf16x8 wx = widen8(now.x[i][e >> 1][(e & 1) * 2], now.x[i][e >> 1][(e & 1) * 2 + 1], now.bx >> (i * 8) & 255u);
+            for (int i = 0; i < 4; i++) {
+                const bf16x8 wx = widen8(now.x[i][e >> 1][(e & 1) * 2], now.x[i][e >> 1][(e & 1) * 2 + 1], now.bx >> (i * 8) & 255u);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp[j], wx, acc[i][j], 0, 0, 0);
-                }
+                for (int j = 0; j < 4; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp[j], wx, acc[i][j], 0, 0, 0);
             }
-        } else {
-#define AE_ONE(I, J) acc[I][J] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(now.p[J][0], now.p[J][1]), join(now.x[I][0], now.x[I][1]), acc[I][J], 0, 0, J, (int)now.bp, I, (int)now.bx);
-#define AE_ROW(I) AE_ONE(I, 0) AE_ONE(I, 1) AE_ONE(I, 2) AE_ONE(I, 3)
-            AE_ROW(0) AE_ROW(1) AE_ROW(2) AE_ROW(3)
-#undef AE_ROW
-#undef AE_ONE
         }
         now = next;
     }
@@ -421,15 +386,16 @@ void launch_tiles(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint3
     check_launch("points8_product");
 }
 
-// 256 x 256 tiles read every operand least often but leave one workgroup on a CU: taken where they fill the chip and their edges waste
-// little (4096 x 4096 x 1024 to bf16: 21.6 against 23.9 us with 128 x 128, 8192^3: 418 against 585; 1024 x 10 000 x 784, 160 tiles: 20.5
-// against 19.4; 300 x 60 000 x 784, two rows of tiles for 300: 35.3 against 30.9).
+// 256 x 256 tiles read every operand least often but leave one workgroup on a CU: taken where they fill the chip several times and their edges waste
+// little (8192 x 16 384 x 4096 to bf16 779 against 915 us with 128 x 128, 8192^3 765 against 895, 8192 x 30 000 x 64 159 against 178; 1024 tiles of four blocks, 8192
+// x 8192 x 512, 78 against 82 and to f32 106 against 101; 4096 x 4096 x 1024, 256 tiles, 32.7 against 33.6 and to f32 40.3 either way; 4096 x 8192 x 256, 512 of
+// them, 27.8 against 25.4; 300 x 60 000 x 784, two rows of tiles for 300, 56 against 44).
 void product(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t ctype, uint64_t ldc, hipStream_t s) {
-    // Workgroups of 64 x 64 that split the coordinates, while each has a CU of its own, or nearly (170 x 258 x 1986 to bf16 8.1 against 11.8 us with 128 x 128 tiles, to f32
-    // 9.7 against 19.9; 1000 x 1000 x 1000, 256 of them, 6.5 against 8.1 and 8.3 against 13.4; 120 x 9069 x 1609, 284, 14.4 against 13.6 and 16.4 against 21.3;
-    // 512 x 4096 x 512, 512, 7.8 against 6.4 and 10.3 against 9.6).
+    // Workgroups of 64 x 64 that split the coordinates, while each has a CU of its own, or nearly (170 x 258 x 1986 to bf16 9.4 against 19.4 us with 128 x 128 tiles; 1000 x
+    // 1000 x 1000, 256 of them, 7.6 against 11.8; 128 x 12 000 x 784, 376, 11.4 against 11.8 and to f32 12.4 against 13.2; 512 x 4096 x 512, 512, 9.0 against 8.3
+    // and 10.9 against 9.7).
     const uint64_t deep_m = (x.rows + 63) / 64, deep_n = (p.rows + 63) / 64;
-    if (deep_m * deep_n <= (ctype == AE_TYPE_F32 ? 384 : 256)) {
+    if (deep_m * deep_n <= 384) {
         const ProductArgs a{x, p, points8_blocks(dim), d_c, ldc, (uint32_t)deep_m, (uint32_t)deep_n, 0};
         by_type(ctype, [&](auto ty) {
             constexpr int TYPE = decltype(ty)::value;
@@ -439,7 +405,7 @@ void product(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t c
         return;
     }
     const uint64_t tm = (x.rows + 255) / 256, tn = (p.rows + 255) / 256;
-    if (tm * tn >= 256 && tm * 256 * 4 <= x.rows * 5 && tn * 256 * 4 <= p.rows * 5) launch_tiles<256, 256, 128>(x, p, dim, d_c, ctype, ldc, s);
+    if (tm * tn >= 1024 && tm * 256 * 4 <= x.rows * 5 && tn * 256 * 4 <= p.rows * 5) launch_tiles<256, 256, 128>(x, p, dim, d_c, ctype, ldc, s);
     else launch_tiles<128, 128, 64>(x, p, dim, d_c, ctype, ldc, s);
 }
 

@@ -604,7 +604,7 @@ int32_t ae_embedder_get_quality_estimate_from_edge_length(const ae_embedder *e, 
  * block, e = the smallest integer >= -126 with a <= 448 * 2^e.  A coordinate is the e4m3 number nearest to x * 2^-e (ties to even); NaN
  * and the infinities are held as NaN.  The scale byte of the block is e + 127.  The value held is code * 2^e.  The scale is a power of two
  * because that costs an 8-bit float none of its relative precision (2^-4), makes x * 2^-e exact (the codes do not depend on how the
- * division is done), makes the value held exact in bf16, and is the scale that the matrix cores multiply by themselves.
+ * division is done) and the value held exact in bf16, which the matrix cores multiply.
  * ------------------------------------------------------------------------------------------------ */
 enum { AE_TYPE_F32 = 0, AE_TYPE_BF16 = 1, AE_TYPE_F16 = 2 };
 typedef struct ae_points8 ae_points8;
@@ -624,10 +624,8 @@ int32_t ae_points8_write(ae_points8 *p, const void *d_x, uint32_t type, uint64_t
    0xFFFFFFFF reads as zeros, any other slot outside the store as NaN. */
 int32_t ae_points8_read(const ae_points8 *p, uint64_t first, const uint32_t *d_slots, uint64_t n, void *d_x, uint32_t type,
                         uint64_t ldx, void *stream);
-/* c[i][j] = <q(x_i), p_{first + j}>, i < m, j < n: the rows x quantised as ae_points8_write would, times the values held, rounded once to
-   `ctype`.  c of f32: exact products, f32 sums.  c of 16 bits: the 8-bit matrix cores, whose sums of eight consecutive products keep 13 bits below
-   the largest of them -- at most 7 * 2^-13 (in the root mean square about 1e-5) of sum_k |x_k p_k|, beside the rounding to 16 bits.  A NaN
-   coordinate makes its products NaN. */
+/* c[i][j] = <q(x_i), p_{first + j}>, i < m, j < n: the rows x quantised as ae_points8_write would, times the values held: exact products, f32
+   sums, rounded once to `ctype`.  A NaN coordinate makes its products NaN. */
 int32_t ae_points8_product(const ae_points8 *p, uint64_t first, uint64_t n, const void *d_x, uint32_t xtype, uint64_t m, uint64_t ldx,
                            void *d_c, uint32_t ctype, uint64_t ldc, void *d_work, uint64_t work_bytes, void *stream);
 int32_t ae_points8_product_work(const ae_points8 *p, uint64_t n, uint64_t m, uint64_t *bytes);
