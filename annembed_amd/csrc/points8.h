@@ -1,6 +1,7 @@
 // points8.h -- points held in 8 bits: the store, its element types, the helpers its kernels share.
 #pragma once
 #include "internal.h"
+#include "points8_plan.h"
 
 struct ae_points8 {
     uint64_t capacity = 0, dim = 0;
@@ -14,8 +15,6 @@ struct ae_points8 {
 
 namespace ae {
 
-constexpr int kBlock = 128;   // coordinates that share a scale
-
 struct Rows8 {   // rows of codes with their scales: part of a store, or quantised rows in scratch memory
     const uint8_t* codes;
     const uint8_t* scales;
@@ -24,8 +23,6 @@ struct Rows8 {   // rows of codes with their scales: part of a store, or quantis
     uint64_t rows;
 };
 
-inline uint64_t points8_row_bytes(uint64_t dim) { return (dim + 15) / 16 * 16; }
-inline uint32_t points8_blocks(uint64_t dim) { return (uint32_t)((dim + kBlock - 1) / kBlock); }
 // bytes from block to block of the scales of `rows` rows, and what lies behind the last one: a tile takes the bytes of rows that do not exist
 // along (they multiply zeros, and no result of theirs is written)
 inline uint64_t points8_scale_stride(uint64_t rows) { return (rows + 15) / 16 * 16; }

@@ -10,18 +10,6 @@ using namespace ae;
 
 namespace {
 
-constexpr int kGroups = 16;    // blocks per workgroup and trip
-constexpr int kTrips = 4;      // blocks a group has in flight: 64 to 128 bytes of loads per lane
-// Up to this many slots a workgroup looks for later occurrences of its rows' slots itself, in one launch, rows of one block up to 4096: 4096 rows of 128 take 6.9
-// us against 7.1 of the two launches otherwise, 8191 of 128 10.1 against 7.1; 5000 of 784 7.3 against 11.1 of three, 8000 of 1500 18.4 against 16.0.
-constexpr uint32_t kScan = 6000;
-
-// Whether a group of lanes takes one block instead of kTrips: fewer loads in flight, more waves.  f32 (32 bytes of loads a lane and block) always, 16 bits up
-// to a million blocks (write 60 000 x 784 of bf16 26 against 30 us, 262 144 x 1024 145 against 148, but read 200 000 x 784 by ids 139 against 116; f32 read
-// 200 000 x 784 137 against 200, write 8191 x 128 scattered 6.8 against 8.1).  Workgroups that look at all slots of the call: while they are few (4096
-// rows of 128 6.9 against 20 us, 4096 rows of 4096 18.5 against 16.2).
-bool spread(uint64_t units, uint32_t type, bool look) { return units <= (look ? 65536 : type == AE_TYPE_F32 ? 1 << 27 : 1 << 20); }
-
 struct Blocks {   // the call's blocks
     uint64_t units, n;
     uint32_t nb;
@@ -190,40 +178,42 @@ Blocks blocks_of(uint64_t n, uint64_t dim) {
     bl.units = n * bl.nb;
     return bl;
 }
-unsigned trips_grid(const Blocks& bl, int trips) {
-    const uint64_t g = (bl.units + kGroups * trips - 1) / (kGroups * trips);
-    if (g * 256 > 0xFFFFFFFFull) fail(AE_ERR_INVALID_ARG, "%llu rows of %u blocks are more than one call takes", (unsigned long long)bl.n, bl.nb);
-    return (unsigned)g;
+BlocksPlan plan_of(uint64_t n, uint64_t dim, uint32_t type, bool look) {
+    const BlocksPlan p = blocks_plan(n, dim, type, look);
+    if (!p.grid) fail(AE_ERR_INVALID_ARG, "%llu rows of %u blocks are more than one call takes", (unsigned long long)n, points8_blocks(dim));
+    return p;
 }
 
 template <int SLOTS>
 void launch_write(const void* d_x, uint32_t type, uint64_t n, uint64_t ldx, uint64_t dim, uint64_t first, const uint32_t* slots, uint32_t* owner, uint64_t capacity,
                   uint8_t* codes, uint8_t* scales, uint64_t scale_stride, hipStream_t s) {
     const Blocks bl = blocks_of(n, dim);
+    const BlocksPlan plan = plan_of(n, dim, type, SLOTS == 1);
     by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         const auto* x = static_cast<const typename Elem<TYPE>::T*>(d_x);
-        auto go = [&](auto kernel, int trips) {
-            hipLaunchKernelGGL(kernel, dim3(trips_grid(bl, trips)), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales, scale_stride);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(plan.grid), dim3(256), 0, s, x, ldx, dim, bl, first, slots, owner, capacity, codes, points8_row_bytes(dim), scales, scale_stride);
         };
-        if (spread(bl.units, type, SLOTS == 1)) go(points8_write_kernel<TYPE, SLOTS, 1>, 1);
-        else go(points8_write_kernel<TYPE, SLOTS, kTrips>, kTrips);
+        if (plan.trips == 1) go(points8_write_kernel<TYPE, SLOTS, 1>);
+        else go(points8_write_kernel<TYPE, SLOTS, kTrips>);
     });
     check_launch("points8_write");
 }
 
 void read_rows(const ae_points8* p, uint64_t first, const uint32_t* slots, uint64_t n, void* d_x, uint32_t type, uint64_t ldx, hipStream_t s) {
     const Blocks bl = blocks_of(n, p->dim);
+    const BlocksPlan plan = plan_of(n, p->dim, type, false);
     by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         auto* x = static_cast<typename Elem<TYPE>::T*>(d_x);
-        auto go = [&](auto kernel, int trips) {
-            hipLaunchKernelGGL(kernel, dim3(trips_grid(bl, trips)), dim3(256), 0, s, (const uint8_t*)p->codes.p, p->row_bytes, (const uint8_t*)p->scales.p, p->scale_stride, p->capacity, first,
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(plan.grid), dim3(256), 0, s, (const uint8_t*)p->codes.p, p->row_bytes, (const uint8_t*)p->scales.p, p->scale_stride, p->capacity, first,
                                slots, bl, x, ldx, p->dim);
         };
-        const bool one = spread(bl.units, type, false);
-        if (slots) one ? go(points8_read_kernel<TYPE, true, 1>, 1) : go(points8_read_kernel<TYPE, true, kTrips>, kTrips);
-        else one ? go(points8_read_kernel<TYPE, false, 1>, 1) : go(points8_read_kernel<TYPE, false, kTrips>, kTrips);
+        const bool one = plan.trips == 1;
+        if (slots) one ? go(points8_read_kernel<TYPE, true, 1>) : go(points8_read_kernel<TYPE, true, kTrips>);
+        else one ? go(points8_read_kernel<TYPE, false, 1>) : go(points8_read_kernel<TYPE, false, kTrips>);
     });
     check_launch("points8_read");
 }
@@ -308,19 +298,24 @@ int32_t ae_points8_write(ae_points8* p, const void* d_x, uint32_t type, uint64_t
         if (n > 0x7FFFFFFFull) fail(AE_ERR_INVALID_ARG, "ae_points8_write: %llu slots are more than one call takes", (unsigned long long)n);
         // The last row of a repeated slot is held.  Few rows: every workgroup looks at the slots behind its own, one launch.  More: the rows claim
         // their slots first and give them back as they are written, or, rows of several blocks, in a launch of their own.
-        if (n <= (p->blocks == 1 ? 4096 : kScan)) {
+        if (write_looks(n, p->dim)) {
             launch_write<1>(d_x, type, n, ldx, p->dim, 0, d_slots, nullptr, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
             return;
         }
+        plan_of(n, p->dim, type, false);   // (a call that is refused claims nothing: what stays claimed would keep later rows out)
         const unsigned grid = blocks_for(n, 256);
         hipLaunchKernelGGL(points8_claim_kernel, dim3(grid), dim3(256), 0, s, d_slots, (uint32_t)n, p->capacity, p->owner.p);
         check_launch("points8_claim");
-        if (p->blocks == 1) {
-            launch_write<3>(d_x, type, n, ldx, p->dim, 0, d_slots, p->owner.p, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
-            return;
+        auto release = [&] { hipLaunchKernelGGL(points8_release_kernel, dim3(grid), dim3(256), 0, s, d_slots, (uint32_t)n, p->capacity, p->owner.p); };
+        try {
+            if (p->blocks == 1) launch_write<3>(d_x, type, n, ldx, p->dim, 0, d_slots, p->owner.p, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
+            else launch_write<2>(d_x, type, n, ldx, p->dim, 0, d_slots, p->owner.p, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
+        } catch (...) {
+            release();
+            throw;
         }
-        launch_write<2>(d_x, type, n, ldx, p->dim, 0, d_slots, p->owner.p, p->capacity, p->codes.p, p->scales.p, p->scale_stride, s);
-        hipLaunchKernelGGL(points8_release_kernel, dim3(grid), dim3(256), 0, s, d_slots, (uint32_t)n, p->capacity, p->owner.p);
+        if (p->blocks == 1) return;
+        release();
         check_launch("points8_release");
     });
 }

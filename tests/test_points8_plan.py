@@ -1,0 +1,61 @@
+"""Which form of a kernel a size takes, and the sizes that are refused: the rules of annembed_amd/csrc/points8_plan.h, compiled for the host."""
+import pathlib
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = pathlib.Path(__file__).resolve().parent.parent
+F32, BF16, F16 = range(3)
+PROGRAM = r"""
+#include "points8_plan.h"
+#include <cinttypes>
+#include <cstdio>
+#include <cstring>
+using namespace ae;
+int main() {
+    char what[16];
+    uint64_t a[8];
+    while (scanf("%15s", what) == 1) {
+        for (auto& v : a)
+            if (scanf("%" SCNu64, &v) != 1) return 1;
+        if (!strcmp(what, "blocks")) {   // n dim type look
+            const BlocksPlan p = blocks_plan(a[0], a[1], (uint32_t)a[2], a[3] != 0);
+            printf("%d %u %d\n", p.trips, p.grid, (int)write_looks(a[0], a[1]));
+        } else return 2;
+    }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no g++")
+    at = tmp_path_factory.mktemp("plan")
+    (at / "plan.cpp").write_text(PROGRAM)
+    subprocess.run([cxx, "-std=c++17", "-Wall", "-Werror", "-O1", "-I", str(ROOT / "annembed_amd" / "csrc"), "-o", str(at / "plan"), str(at / "plan.cpp")], check=True)
+
+    def ask(what, *numbers):
+        line = " ".join([what] + [str(int(v)) for v in numbers] + ["0"] * (8 - len(numbers)))
+        out = subprocess.run([str(at / "plan")], input=line + "\n", capture_output=True, text=True, check=True).stdout
+        return tuple(int(v) if v.lstrip("-").isdigit() else float(v) for v in out.split())
+    return ask
+
+
+def test_launches_of_2_to_the_32_threads_are_refused(plan):
+    """a workgroup of 256 threads takes 64 blocks of 16-bit rows, and of f32 beyond 2^27: 2^30 - 64 blocks are the most"""
+    for kind in (F32, BF16, F16):
+        assert plan("blocks", (1 << 30) - 64, 128, kind, 0)[:2] == (4, (1 << 24) - 1)
+        for n, dim in (((1 << 30) - 63, 1), (1 << 30, 128), ((1 << 29) - 31, 129), ((1 << 31) - 1, 5), (1 << 20, 1 << 20)):
+            assert plan("blocks", n, dim, kind, 0)[1] == 0
+    assert plan("blocks", 1, 1, F32, 0)[:2] == (1, 1) and plan("blocks", 17, 128, BF16, 0)[:2] == (1, 2)
+
+
+def test_blocks_a_group_of_lanes_takes(plan):
+    assert plan("blocks", (1 << 20) - 5, 16, BF16, 0)[0] == 1 and plan("blocks", (1 << 20) + 77, 16, F16, 0)[0] == 4
+    assert plan("blocks", (1 << 19) + 5, 130, BF16, 0)[0] == 4 and plan("blocks", 150001, 1000, BF16, 0)[0] == 4 and plan("blocks", 150001, 1000, F32, 0)[0] == 1
+    assert plan("blocks", 4001, 1000, BF16, 1) == (1, 2001, 1) and plan("blocks", 5000, 4096, BF16, 1)[0] == 4
+    for n, dim, looks in ((4096, 128, 1), (4097, 128, 0), (6000, 129, 1), (6001, 129, 0)):
+        assert plan("blocks", n, dim, BF16, 0)[2] == looks
