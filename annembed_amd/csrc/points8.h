@@ -135,7 +135,8 @@ __device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
     }
     return a;
 }
-// the codes of eight values under a scale byte.  x * 2^-e is exact (or below every code), |.| <= 448: one rounding, the conversion's
+// the codes of eight values under a scale byte.  x * 2^-e is exact (or below every code), |.| <= 448: one rounding, the conversion's.  Under the largest
+// scale, 2^120, the codes from 256 on would stand for 2^128 and more, which f32 does not have: 240 is the largest there, what is finite stays finite.
 __device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t byte) {
     const float shrink = __uint_as_float((254u - byte) << 23);
     float y[8];
@@ -143,6 +144,10 @@ __device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t byte) {
     for (int t = 0; t < 8; t++) {
         const bool finite = (__float_as_uint(v[t]) & 0x7FFFFFFFu) < 0x7F800000u;
         y[t] = finite ? v[t] * shrink : __uint_as_float(0x7FC00000u);
+    }
+    if (byte == 247u) {
+#pragma unroll
+        for (int t = 0; t < 8; t++) y[t] = y[t] != y[t] ? y[t] : __builtin_amdgcn_fmed3f(y[t], -240.f, 240.f);
     }
     int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
@@ -159,7 +164,7 @@ __device__ __forceinline__ void decode8(uint2 c, uint32_t byte, float (&v)[8]) {
     v[4] = d[0] * scale; v[5] = d[1] * scale; v[6] = e[0] * scale; v[7] = e[1] * scale;
 }
 
-// the values of eight codes as bf16, exact: widened with the block's power of two in one step
+// the values of eight codes as bf16, exact (to a multiple of 2^-133, its smallest number): widened with the block's power of two in one step
 __device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi, uint32_t byte) {
     using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
     const float scale = __uint_as_float(byte << 23);

@@ -601,8 +601,8 @@ int32_t ae_embedder_get_quality_estimate_from_edge_length(const ae_embedder *e, 
  * Sizes that need 2^32 threads or more in one launch are refused.
  *
  * Format: a row of `dim` coordinates in blocks of 128 (the last may be shorter).  a = the largest magnitude among the finite values of the
- * block, e = the smallest integer >= -126 with a <= 448 * 2^e.  A coordinate is the e4m3 number nearest to x * 2^-e (ties to even); NaN
- * and the infinities are held as NaN.  The scale byte of the block is e + 127.  The value held is code * 2^e.  The scale is a power of two
+ * block, e = the smallest integer >= -126 with a <= 448 * 2^e.  A coordinate is the e4m3 number nearest to x * 2^-e (ties to even) whose value
+ * f32 has: where e = 120 the largest is 240, and magnitudes from 248 * 2^120 on are held as 240 * 2^120; NaN and the infinities are held as NaN.  The scale byte of the block is e + 127.  The value held is code * 2^e.  The scale is a power of two
  * because that costs an 8-bit float none of its relative precision (2^-4), makes x * 2^-e exact (the codes do not depend on how the
  * division is done) and the value held exact in bf16, which the matrix cores multiply.
  * ------------------------------------------------------------------------------------------------ */
@@ -625,7 +625,7 @@ int32_t ae_points8_write(ae_points8 *p, const void *d_x, uint32_t type, uint64_t
 int32_t ae_points8_read(const ae_points8 *p, uint64_t first, const uint32_t *d_slots, uint64_t n, void *d_x, uint32_t type,
                         uint64_t ldx, void *stream);
 /* c[i][j] = <q(x_i), p_{first + j}>, i < m, j < n: the rows x quantised as ae_points8_write would, times the values held: exact products, f32
-   sums, rounded once to `ctype`.  A NaN coordinate makes its products NaN. */
+   sums, rounded once to `ctype`.  (Values held below 2^-126 enter as the nearest multiple of 2^-133.)  A NaN coordinate makes its products NaN. */
 int32_t ae_points8_product(const ae_points8 *p, uint64_t first, uint64_t n, const void *d_x, uint32_t xtype, uint64_t m, uint64_t ldx,
                            void *d_c, uint32_t ctype, uint64_t ldc, void *d_work, uint64_t work_bytes, void *stream);
 int32_t ae_points8_product_work(const ae_points8 *p, uint64_t n, uint64_t m, uint64_t *bytes);
@@ -633,7 +633,7 @@ int32_t ae_points8_product_work(const ae_points8 *p, uint64_t n, uint64_t m, uin
 int32_t ae_points8_product_points(const ae_points8 *p, uint64_t first, uint64_t n, const ae_points8 *q, uint64_t q_first, uint64_t m,
                                   void *d_c, uint32_t ctype, uint64_t ldc, void *stream);
 /* The gradient of ae_points8_product to its rows, q taken as the identity: dx[i][k] = sum_j dc[i][j] * p_{first + j}[k].  dc enters exactly
-   whatever its type (but for what lies below 2^-126), sums are f32 in an order that equal calls share. */
+   whatever its type (but for what lies below 2^-126), values held as in the product, sums are f32 in an order that equal calls share. */
 int32_t ae_points8_product_grad(const ae_points8 *p, uint64_t first, uint64_t n, const void *d_dc, uint32_t dctype, uint64_t m,
                                 uint64_t lddc, void *d_dx, uint32_t xtype, uint64_t lddx, void *d_work, uint64_t work_bytes, void *stream);
 int32_t ae_points8_product_grad_work(const ae_points8 *p, uint64_t n, uint64_t m, uint32_t dctype, uint64_t *bytes);
