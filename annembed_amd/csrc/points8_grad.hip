@@ -97,14 +97,14 @@ __device__ __forceinline__ bool place_of(const GradArgs& a, uint32_t& slice, uin
     return true;
 }
 
-// dc of f32 and f16 (and of any type whose rows lie too far apart for 32-bit offsets, or that ends in half a dword with its page).  A wave owns 16 FR of
+// dc of f32 and f16 (and of any type whose rows lie too far apart for 32-bit offsets).  A wave owns 16 FR of
 // the rows and all coordinates, so each value of dc is split once.  dc goes to LDS as it is, three steps deep.  (Straight to the lanes that
 // multiply it, 16 bytes of 16 rows each, every lane would be an access of its own to the cache.)  The codes are turned on the way to LDS: a thread takes
 // 4 coordinates of 8 points, widens them under the products of the step before and writes 8 points of one coordinate as 16 bytes.  One
 // barrier a step.  8192 x 8192 x 4096 of f32: 970 TF of the three partial products, at the rate of the matrix cores; 300 x 60 000 x 784: 107 us.
 template <int TYPE, int FR> constexpr int grad_lds() { return 3 * 64 * FR * kStep * (TYPE == AE_TYPE_F32 ? 4 : 2) + 2 * kBlock * 128; }   // 56 or 80 KB: two workgroups a CU
 
-template <int TYPE, int FR, bool VEC>   // VEC: the copies' 32-bit offsets and whole pieces do for dc
+template <int TYPE, int FR, bool VEC>   // VEC: the copies' 32-bit offsets do for dc
 __global__ void __launch_bounds__(256, 2) grad_tile_kernel(GradArgs a) {
     using T = typename Elem<TYPE>::T;
     constexpr int TERMS = terms_of<TYPE>(), ROW = kStep * (int)sizeof(T), PIECES = ROW / 16, STAGE = 64 * FR * ROW, COPIES = STAGE / 4096;
@@ -118,11 +118,11 @@ __global__ void __launch_bounds__(256, 2) grad_tile_kernel(GradArgs a) {
     const uint32_t mi = (uint32_t)min((uint64_t)(64 * FR), a.m - i0), points = (uint32_t)(je - jb), steps = (points + kStep - 1) / kStep;
     const int r0 = wave * 16 * FR + (lane & 15);   // this lane's first row of the tile; the others 16 apart
     const T* dc = static_cast<const T*>(a.dc) + i0 * a.lddc + jb;
-    // Rows beyond m lie outside the buffer's range, which ends with the dword of the last row's last point (what of a piece lies behind it reads as
-    // 0).  A lane's offsets never change, the step goes into the scalar one, which stays inside the range (steps past the last one fetch the last
-    // again, for nobody).  What is fetched behind the last point is cut in the last step.
+    // Rows beyond m lie outside the buffer's range, which ends with the last row's last point: dwords that are not wholly inside read as 0, so an odd 16-bit
+    // value at the very end is put in by itself in the last step, where what is fetched behind the other rows' last point is cut.  A lane's offsets
+    // never change, the step goes into the scalar one, which stays inside the range (steps past the last one fetch the last again, for nobody).
     const uint32_t row_bytes = (uint32_t)a.lddc * (uint32_t)sizeof(T);
-    __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)dc, (short)0, VEC ? (int)((mi - 1) * row_bytes + (points * (uint32_t)sizeof(T) + 3) / 4 * 4) : 0, 0x00027000);
+    __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)dc, (short)0, VEC ? (int)grad_range(mi, row_bytes, points, sizeof(T)) : 0, 0x00027000);
     __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.codes + jb * a.p.row_bytes), (short)0, (int)(points * (uint32_t)a.p.row_bytes), 0x00027000);
     const uint32_t k_at = (uint32_t)k0 + kg * 4, code_at = (uint32_t)(jg * 8) * (uint32_t)a.p.row_bytes + (k_at < a.p.row_bytes ? k_at : kOutside);
     const uint8_t* sc = a.p.scales + tk * a.p.scale_stride + jb + jg * 8;
@@ -189,6 +189,7 @@ __global__ void __launch_bounds__(256, 2) grad_tile_kernel(GradArgs a) {
             }
     };
     uint32_t stage = 0;   // of this step's dc
+    T final = (T)0.f;     // the last row's last point
     // A step is 16 parts: 16 coordinates over a half of the points.  Everything is read two parts ahead.  Two parts before its end a step's dc and
     // coordinates have been read by everybody and the next one's have to be there.
     auto step = [&](uint32_t t, auto which, auto last) {
@@ -217,7 +218,11 @@ __global__ void __launch_bounds__(256, 2) grad_tile_kernel(GradArgs a) {
                     __builtin_memcpy(v, raw[x >> 3][i], sizeof(v));
                     if constexpr (VEC && LAST) {   // cut what lies behind the last point
 #pragma unroll
-                        for (int e = 0; e < 8; e++) v[e] = t * kStep + part(x >> 3, g) * 8 + e < points ? v[e] : (T)0.f;
+                        for (int e = 0; e < 8; e++) {
+                            const uint32_t j = t * kStep + part(x >> 3, g) * 8 + e;
+                            v[e] = j < points ? v[e] : (T)0.f;
+                            if constexpr (sizeof(T) == 2) v[e] = j == points - 1 && (uint32_t)(r0 + i * 16) == mi - 1 ? final : v[e];
+                        }
                     }
                     split8<TYPE>(v, terms[i]);
                 }
@@ -253,6 +258,7 @@ __global__ void __launch_bounds__(256, 2) grad_tile_kernel(GradArgs a) {
         step(t, even, std::false_type{});
         step(t + 1, odd, std::false_type{});
     }
+    if constexpr (VEC && sizeof(T) == 2) final = dc[(mi - 1) * a.lddc + points - 1];
     if (t + 1 < steps) {
         step(t, even, std::false_type{});
         step(t + 1, odd, std::true_type{});
@@ -291,7 +297,7 @@ __global__ void __launch_bounds__(256, 2) grad_turn_kernel(GradArgs a) {
     const __bf16* dc = static_cast<const __bf16*>(a.dc) + i0 * a.lddc + jb;
     // ---- the copies.  Ranges and what lies behind the last point: as above
     const uint32_t row_bytes = (uint32_t)a.lddc * 2, stride = (uint32_t)a.p.row_bytes;
-    __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)dc, (short)0, (int)((mi - 1) * row_bytes + (points * 2 + 3) / 4 * 4), 0x00027000);
+    __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)dc, (short)0, (int)grad_range(mi, row_bytes, points, 2), 0x00027000);
     __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.codes + jb * stride), (short)0, (int)(points * stride), 0x00027000);
     __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.scales + tk * a.p.scale_stride + jb), (short)0, (int)(points + 256), 0x00027000);   // (kScaleSlack)
     const int copy_row = wave * 8 + (lane >> 3), copy_piece = (lane & 7) ^ turn<8>(copy_row);
@@ -346,7 +352,8 @@ __global__ void __launch_bounds__(256, 2) grad_turn_kernel(GradArgs a) {
     for (int i = 0; i < FR; i++)
 #pragma unroll
         for (int f = 0; f < 4; f++) acc[i][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    uint32_t stage = 0;   // of this step
+    uint32_t stage = 0;             // of this step
+    __bf16 final = (__bf16)0.f;   // the last row's last point
     auto step = [&](uint32_t t, auto which, auto last) {
         constexpr int S = decltype(which)::value;
         constexpr bool LAST = decltype(last)::value;
@@ -370,7 +377,11 @@ __global__ void __launch_bounds__(256, 2) grad_turn_kernel(GradArgs a) {
             bf16x8 v = __builtin_bit_cast(bf16x8, rows[(S * FR + i) & 3]);
             if constexpr (LAST) {   // cut what lies behind the last point
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = t * kStep + mine * 8 + e < points ? v[e] : (__bf16)0.f;
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t j = t * kStep + mine * 8 + e;
+                    v[e] = j < points ? v[e] : (__bf16)0.f;
+                    v[e] = j == points - 1 && (uint32_t)(i * 16 + (lane & 15)) == mi - 1 ? final : v[e];
+                }
             }
 #pragma unroll
             for (int f = 0; f < 4; f++) acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, frag[S][f]), v, acc[i][f], 0, 0, 0);
@@ -408,6 +419,7 @@ __global__ void __launch_bounds__(256, 2) grad_turn_kernel(GradArgs a) {
         step(t, even, std::false_type{});
         step(t + 1, odd, std::false_type{});
     }
+    final = dc[(mi - 1) * a.lddc + points - 1];
     step(t, even, std::false_type{});
     step(t + 1, odd, std::true_type{});
     // ---- the two halves of the points, through LDS (the copies for nobody have ended first)
@@ -548,10 +560,7 @@ int32_t ae_points8_product_grad(const ae_points8* p, uint64_t first, uint64_t n,
             const uint64_t tiles = g.tiles_m * g.tiles_k;
             GradArgs a{d_dc, lddc, m, n, p->dim, points8_rows(p, first, n), g.per_slice, (float*)d_work, g.ldp, (uint32_t)g.tiles_k, (uint32_t)tiles, (uint32_t)g.slices, d_dx, xtype, lddx};
             const unsigned grid = (unsigned)((tiles * g.slices + 7) / 8 * 8);
-            // The copies take 16 bytes at any address and the dwords that the buffer's range holds whole.  The last of an odd number of 16-bit values is the
-            // first half of a dword: the range then goes 2 bytes past it, which must not be the next page.
-            const uint64_t size = type_size(dctype), end = (uint64_t)(uintptr_t)d_dc + ((m - 1) * lddc + n) * size;
-            const bool vec = lddc * size < 0x3FFF0000ull / (64 * g.fr) && (n * size % 4 == 0 || end % 4096 != 0);
+            const bool vec = lddc * type_size(dctype) < 0x3FFF0000ull / (64 * g.fr);
             by_type(dctype, [&](auto ty) {
                 constexpr int TYPE = decltype(ty)::value;
                 if (g.fr == 1) launch_grad<TYPE, 1>(a, vec, grid, s);

@@ -39,4 +39,9 @@ inline BlocksPlan blocks_plan(uint64_t n, uint64_t dim, uint32_t type, bool look
     return p;
 }
 
+// ---- the gradient of the product
+
+// bytes of dc from a tile's first value to its last one in a slice of the points, and not one more: what a 16-byte piece has behind them is not fetched
+constexpr uint32_t grad_range(uint32_t rows, uint32_t row_bytes, uint32_t points, uint32_t size) { return (rows - 1) * row_bytes + points * size; }
+
 }  // namespace ae

@@ -1,4 +1,4 @@
-"""The two ends of f32's range in the 8-bit store: what is finite stays finite and multiplies as such; the smallest values."""
+"""The ends of things in the 8-bit store: of f32's range, where what is finite stays finite and multiplies as such, and of a tensor's memory."""
 import numpy as np
 import pytest
 import torch
@@ -81,3 +81,25 @@ def test_the_smallest_values(A, m):
     dc[:, :300] = scale
     grad = bank.product_grad(dc.cuda()).cpu().double().numpy()
     assert (np.abs(grad[:, 5] - scale * want[:, 5].sum()) <= scale * (300 * 2.0 ** -134 + 300 * 2.0 ** -24 * want[:, 5].sum())).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,dim", [(1, 1, 1), (1, 65, 130), (5, 129, 40), (64, 4097, 28), (65, 63, 200), (300, 5001, 784), (130, 70001, 131), (2100, 3001, 130)])
+def test_the_last_value_of_dc_counts(A, m, n, dim, dtype):
+    """an odd number of values, the last ones of their memory and of a page, and beside NaN: sums of small integers are exact"""
+    rng = np.random.default_rng(n)
+    p, dc = rng.integers(-7, 8, (n, dim)).astype(np.float32), rng.integers(-7, 8, (m, n)).astype(np.float32)
+    p[-1], dc[:, -1] = 7, 5
+    want = torch.from_numpy(dc @ p)
+    bank = A.Points8(n, dim)
+    bank.write(torch.from_numpy(p).cuda())
+    src = torch.from_numpy(dc).to(dtype).cuda()
+    size = src.element_size()
+    room = torch.full((m * n + 3 * 4096 // size,), float("nan"), dtype=dtype, device="cuda")
+    end = (-(room.data_ptr() + m * n * size) % 4096 + 4096) // size + m * n   # elements to an end of a page behind m * n
+    for last in (end, end - 1, end + 1):
+        view = room[last - m * n:last].view(m, n)
+        view.copy_(src)
+        assert (view.data_ptr() + m * n * size) % 4096 == (last - end) * size % 4096
+        assert torch.equal(bank.product_grad(view).cpu(), want)
+        room.fill_(float("nan"))

@@ -22,6 +22,8 @@ int main() {
         if (!strcmp(what, "blocks")) {   // n dim type look
             const BlocksPlan p = blocks_plan(a[0], a[1], (uint32_t)a[2], a[3] != 0);
             printf("%d %u %d\n", p.trips, p.grid, (int)write_looks(a[0], a[1]));
+        } else if (!strcmp(what, "range")) {   // rows lddc points size
+            printf("%u\n", grad_range((uint32_t)a[0], (uint32_t)(a[1] * a[3]), (uint32_t)a[2], (uint32_t)a[3]));
         } else return 2;
     }
 }
@@ -59,3 +61,9 @@ def test_blocks_a_group_of_lanes_takes(plan):
     assert plan("blocks", 4001, 1000, BF16, 1) == (1, 2001, 1) and plan("blocks", 5000, 4096, BF16, 1)[0] == 4
     for n, dim, looks in ((4096, 128, 1), (4097, 128, 0), (6000, 129, 1), (6001, 129, 0)):
         assert plan("blocks", n, dim, BF16, 0)[2] == looks
+
+
+def test_the_gradient_reads_nothing_behind_its_tensor(plan):
+    """a tile's buffer ends with its last row's last value, whether that is a whole dword or the first half of one"""
+    for rows, lddc, points, size in ((1, 1, 1, 2), (1, 129, 129, 2), (64, 129, 129, 2), (128, 60001, 60001, 2), (5, 140, 129, 2), (64, 7, 7, 4), (3, 64, 64, 2)):
+        assert plan("range", rows, lddc, points, size)[0] == ((rows - 1) * lddc + points) * size
