@@ -11,8 +11,9 @@ softmax of its scores against the bank follows the graph's edge probabilities.
     dq = bank.product_grad(dlogits)                        # [m, dim]
 
 Tensors live on one GPU; the work goes to torch's current stream of that GPU and the calls return at once: they neither synchronise nor
-allocate outside torch's allocator, so they can be captured into a graph.  The formats, formulas and edge cases are those of ae_points8_* and
-ae_teacher_* in include/annembed_hip.h.
+allocate outside torch's allocator, so they can be captured into a graph (which keeps neither the store nor the caller's tensors alive).  Results are
+detached: gradients are the calls product_grad and teacher_loss / teacher_grad.  A tensor of the caller's that a call writes to counts as changed in
+place, and so do codes() and scales() at every write.  The formats, formulas and edge cases are those of ae_points8_* and ae_teacher_* in include/annembed_hip.h.
 """
 import ctypes as C
 import functools
@@ -91,6 +92,10 @@ def _loss_work(rows, cols):
     return need.value
 
 
+# what is written behind torch's back has another version, so that autograd refuses to go back through what it held before
+_changed = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version   # (of a list; the public one looks at it first)
+
+
 class _Store:
     """the handle, and the bytes of scratch of its calls, asked for once for each size; views of its memory keep it alive"""
 
@@ -142,6 +147,7 @@ class Points8:
             c = torch.as_tensor(_View(self._store, codes.value, (self.capacity, self.dim), (row_bytes.value, 1)), device=self.device)
             self._codes = c.view(torch.float8_e4m3fn)
             self._scales = torch.as_tensor(_View(self._store, scales.value, (self.capacity, blocks), (1, stride.value)), device=self.device)
+            self._views = [self._codes, self._scales]
 
     @property
     def handle(self):
@@ -171,6 +177,7 @@ class Points8:
         s = _vector(slots, "slots", self.device, n, _INDEX)
         n, first = (n, 0) if slots is not None else self._range(n, first)
         _call(self.device, "ae_points8_write", self._store.h, p, ty, n, ld, first, s if n else None)
+        _changed(self._views)
 
     def read(self, n=None, first=0, slots=None, dtype=torch.float32, out=None):
         """the values held in points first ... first + n - 1, or in `slots` (-1 reads as zeros, others outside the store as NaN)"""
@@ -182,10 +189,13 @@ class Points8:
         else:
             n, first = self._range(n, first)
         s = _vector(slots, "slots", self.device, n, _INDEX)
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty(n, self.dim, dtype=dtype, device=self.device)
         p, ty, ld = _rows(out, "out", self.device, (n, self.dim))
         _call(self.device, "ae_points8_read", self._store.h, first, s if n else None, n, p, ty, ld)
+        if given:
+            _changed([out])
         return out
 
     def _work(self, work, need):
@@ -205,14 +215,17 @@ class Points8:
             m = x.shape[0]
             if x.shape[1] != self.dim:
                 raise _bad("x has %d coordinates, the store %d" % (x.shape[1], self.dim))
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty(m, n, dtype=dtype, device=self.device)
         p, ty, ld = _rows(out, "out", self.device, (m, n))
         if isinstance(x, Points8):
             _call(self.device, "ae_points8_product_points", self._store.h, first, n, x._store.h, x_first, m, p, ty, ld)
-            return out
-        wp, wn, keep = self._work(work, self._store.product_work(n, m))
-        _call(self.device, "ae_points8_product", self._store.h, first, n, xp, xt, m, xl, p, ty, ld, wp, wn)
+        else:
+            wp, wn, keep = self._work(work, self._store.product_work(n, m))
+            _call(self.device, "ae_points8_product", self._store.h, first, n, xp, xt, m, xl, p, ty, ld, wp, wn)
+        if given:
+            _changed([out])
         return out
 
     def product_grad(self, dc, n=None, first=0, dtype=torch.float32, out=None, work=None):
@@ -222,11 +235,14 @@ class Points8:
         m = dc.shape[0]
         if dc.shape[1] != n:
             raise _bad("dc has %d columns for %d points" % (dc.shape[1], n))
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty(m, self.dim, dtype=dtype, device=self.device)
         p, ty, ld = _rows(out, "out", self.device, (m, self.dim))
         wp, wn, keep = self._work(work, self._store.product_grad_work(n, m, dt))
         _call(self.device, "ae_points8_product_grad", self._store.h, first, n, dp, dt, m, dl, p, ty, ld, wp, wn)
+        if given:
+            _changed([out])
         return out
 
 
@@ -289,6 +305,8 @@ def teacher_loss(logits, idx, values, teacher="proba", temperature=1.0, row_weig
         raise _bad("work has to be a contiguous tensor on %s" % device)
     _call(device, "ae_teacher_loss", p, ty, rows, cols, ld, ip, vp, k, ldk, _kind(teacher), float(temperature), wp, loss.data_ptr(), stats.data_ptr(), gp, gl,
           None if work is None else work.data_ptr(), 0 if work is None else work.numel() * work.element_size())
+    if g is not None and grad is not True:
+        _changed([g])
     return (loss, stats) if g is None else (loss, stats, g)
 
 
@@ -307,4 +325,6 @@ def teacher_grad(logits, stats, idx, values, dloss=None, teacher="proba", temper
     if gt != ty:
         raise _bad("out is %s, the logits %s" % (g.dtype, logits.dtype))
     _call(device, "ae_teacher_grad", p, ty, rows, cols, ld, stats.data_ptr(), ip, vp, k, ldk, _kind(teacher), float(temperature), up, gp, gl)
+    if out is not None:
+        _changed([g])
     return g
