@@ -212,6 +212,8 @@ class Points8:
             m, x_first = x._range(m, x_first)
         else:
             xp, xt, xl = _rows(x, "x", self.device)
+            if x_first != 0 or m not in (None, x.shape[0]):
+                raise _bad("x_first and m choose points of another store: of a tensor all %d rows are taken" % x.shape[0])
             m = x.shape[0]
             if x.shape[1] != self.dim:
                 raise _bad("x has %d coordinates, the store %d" % (x.shape[1], self.dim))

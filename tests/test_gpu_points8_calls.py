@@ -56,3 +56,13 @@ def test_autograd_sees_what_is_written(A):
         t = torch.zeros(6, 20, device="cuda")
         A.teacher_loss(w, idx, p, grad=t)
         assert t.any()
+
+
+def test_rows_of_a_tensor_are_all_taken(A):
+    """m and x_first choose points of another store: with a tensor they would be passed over, so they are refused"""
+    bank = A.Points8(40, 30)
+    x = torch.ones(5, 30, device="cuda")
+    for more in (dict(m=3), dict(m=6), dict(x_first=1), dict(x_first=1, m=4)):
+        with pytest.raises(A.AnnembedError):
+            bank.product(x, **more)
+    assert bank.product(x, m=5, x_first=0).shape == (5, 40)
