@@ -222,13 +222,14 @@ __global__ void __launch_bounds__(256) knn_refine_kernel(const float* __restrict
         f += df * df;
     }
     if (!valid) f = INFINITY;
-    // rank of (f, j) among the 32 candidates of the row (j: the caller's id where the points were reordered internally -- `orig`)
+    // rank of (f, j) among the 32 candidates of the row (j: the caller's id where the points were reordered internally -- `orig`); empty places, which
+    // are alike, by their place: every rank is one lane's, whatever the row holds (NaN, or norms beyond f32, leave places empty)
     const uint32_t jt = (orig && valid) ? orig[j] : j;
     int rank = 0;
     for (int o = 0; o < kM; o++) {
         const float fo = __shfl(f, o, kM);
         const uint32_t jo = (uint32_t)__shfl((int)jt, o, kM);
-        rank += (fo < f || (fo == f && jo < jt)) ? 1 : 0;
+        rank += (fo < f || (fo == f && (jo < jt || (jo == jt && o < s)))) ? 1 : 0;
     }
     if ((uint32_t)rank < k) {
         nbr[orow * k + rank] = j;

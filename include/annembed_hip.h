@@ -638,7 +638,8 @@ int32_t ae_points8_product_grad(const ae_points8 *p, uint64_t first, uint64_t n,
                                 uint64_t lddc, void *d_dx, uint32_t xtype, uint64_t lddx, void *d_work, uint64_t work_bytes, void *stream);
 int32_t ae_points8_product_grad_work(const ae_points8 *p, uint64_t n, uint64_t m, uint32_t dctype, uint64_t *bytes);
 /* ae_kgraph_bruteforce_l2 of the values held in rows first ... first + n - 1: exact neighbours and distances of the points as the store has
-   them (they are read back in f32 on the device, never through the host).  Waits for `stream`, where the rows were written. */
+   them (they are read back in f32 on the device, never through the host: n * dim * 4 bytes while it runs).  A point with a NaN coordinate is nobody's
+   neighbour and has none, which is refused.  Waits for `stream`, where the rows were written. */
 int32_t ae_kgraph_bruteforce_l2_points8(const ae_points8 *p, uint64_t first, uint64_t n, uint32_t nbng, void *stream, ae_kgraph **out);
 
 /* Cross entropy of rows of logits against a teacher's top list, relative to the teacher's own entropy (a Kullback-Leibler divergence
