@@ -517,6 +517,7 @@ int32_t ae_teacher_loss(const void* d_logits, uint32_t type, uint64_t rows, uint
         if (!d_loss || !d_stats) fail(AE_ERR_INVALID_ARG, "ae_teacher_loss: loss or stats is NULL");
         check_aligned(d_loss, 4, "ae_teacher_loss: loss");
         check_aligned(d_stats, 4, "ae_teacher_loss: stats");
+        check_aligned(d_row_weight, 4, "ae_teacher_loss: row weights");
         require_device();
         const Call a{d_logits, type, rows, cols, ld, TeacherList{d_idx, d_list, ldk, k, kind}, temperature, d_row_weight, d_loss, d_stats, d_grad, ldg, (hipStream_t)stream};
         // Where the gradient is wanted too the row held in registers saves a read (300 x 60 000 of f32: 52 us either way, 600: 88 against 115).  For the loss
@@ -542,6 +543,7 @@ int32_t ae_teacher_grad(const void* d_logits, uint32_t type, uint64_t rows, uint
         if (d_grad == d_logits && ldg != ld) fail(AE_ERR_INVALID_ARG, "ae_teacher_grad: a gradient in place has the logits' stride");
         if (!d_stats) fail(AE_ERR_INVALID_ARG, "ae_teacher_grad: stats is NULL");
         check_aligned(d_stats, 4, "ae_teacher_grad: stats");
+        check_aligned(d_dloss, 4, "ae_teacher_grad: dloss");
         require_device();
         const Call a{d_logits, type, rows, cols, ld, TeacherList{d_idx, d_list, ldk, k, kind}, temperature, d_dloss, nullptr, const_cast<float*>(d_stats), d_grad, ldg, (hipStream_t)stream};
         // nothing to hold: slices from 16 384 logits on (300 x 60 000 of f32: 33 against 37 us, 2000 x 16 384: 49 against 60)
