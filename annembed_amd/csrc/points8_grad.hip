@@ -12,7 +12,6 @@ using namespace ae;
 
 namespace {
 
-constexpr int kStep = 64;    // points per step: 128 bytes of bf16
 constexpr uint32_t kPast = 0x3FFF0000u;      // the ranges of a tile's rows of dc and of a slice's codes do not reach this far
 constexpr uint32_t kOutside = 0x40000000u;   // an offset outside every buffer's range (dc's rows of a tile, a slice's codes: less than 1 GiB)
 
@@ -482,40 +481,6 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const float* __restrict_
         if (k + t < dim) dx[i * lddx + k + t] = (typename Elem<TYPE>::T)s[t];
 }
 
-struct GradPlan {
-    uint32_t fr;   // 64 rows of dc a tile, or 128
-    uint64_t tiles_m, tiles_k, slices, per_slice, ldp, bytes;
-};
-GradPlan grad_plan(uint64_t m, uint64_t n, uint64_t dim, uint32_t dctype) {
-    GradPlan best{};
-    const uint64_t steps = std::max<uint64_t>((n + kStep - 1) / kStep, 1), tiles_k = (dim + kBlock - 1) / kBlock, ldp = (dim + 3) / 4 * 4;
-    const uint64_t most = 0x3FFF0000ull / points8_row_bytes(dim) / kStep, least_slices = (steps + most - 1) / most;   // a slice's codes: less than 1 GiB
-    // What a choice costs, in us: a workgroup's beginning and end; its steps, with so many workgroups on a CU (measured at 300 x 60 000 x 784, between operands
-    // in cache and operands from memory; more workgroups do not fit or do not pay); the slices' sums, written and read again at 5 TB/s; the launch that
-    // joins them.  bf16, from memory: 300 x 60 000 x 784 56 us with 128 rows and two workgroups on a CU, 58 to 65 otherwise; 64 rows of it 22.4 with 64
-    // and one, 24 to 27 otherwise; 1000 x 1000 x 1000 in one slice 12.6 against 16 to 21 in several.
-    struct Choice { uint32_t fr, wgs; float step; };
-    static constexpr Choice bf16[] = {{1, 1, 0.43f}, {1, 2, 0.66f}, {2, 1, 0.55f}, {2, 2, 0.86f}};
-    static constexpr Choice f16[] = {{1, 1, 0.84f}, {1, 2, 1.1f}, {2, 1, 1.25f}, {2, 2, 1.76f}};
-    static constexpr Choice f32[] = {{1, 1, 1.07f}, {1, 2, 1.46f}};
-    const Choice* const choices = dctype == AE_TYPE_BF16 ? bf16 : dctype == AE_TYPE_F16 ? f16 : f32;
-    const int count = dctype == AE_TYPE_F32 ? 2 : 4;
-    double least = 0.;
-    for (int q = 0; q < count; q++) {
-        const Choice& c = choices[q];
-        const uint64_t tiles_m = (m + 64 * c.fr - 1) / (64 * c.fr), tiles = tiles_m * tiles_k, slots = 256 * c.wgs;
-        for (const uint64_t want : {(uint64_t)1, slots / tiles}) {
-            const uint64_t slices = std::max<uint64_t>({1, least_slices, std::min(want, (steps + 3) / 4)}), per = (steps + slices - 1) / slices, used = (steps + per - 1) / per;
-            const double rounds = (double)((tiles * used + slots - 1) / slots);
-            const double cost = rounds * ((c.fr == 1 ? 2 : 5) + per * c.step) + (used > 1 ? 4. + used * (0.005 + m * ldp * 8 / 5.1e6) : 0.);
-            if (best.fr && cost >= least) continue;
-            least = cost;
-            best = GradPlan{c.fr, tiles_m, tiles_k, used, per * kStep, ldp, used > 1 ? used * m * ldp * 4 : 0};
-        }
-    }
-    return best;
-}
-
 template <int TYPE, int FR>
 void launch_grad(const GradArgs& a, bool vec, unsigned grid, hipStream_t s) {
     if (!vec) hipLaunchKernelGGL((grad_tile_kernel<TYPE, FR, false>), dim3(grid), dim3(256), (grad_lds<TYPE, FR>()), s, a);
@@ -552,7 +517,7 @@ int32_t ae_points8_product_grad(const ae_points8* p, uint64_t first, uint64_t n,
         if (g.bytes && (!d_work || work_bytes < g.bytes))
             fail(AE_ERR_INVALID_ARG, "ae_points8_product_grad: %llu bytes of scratch are needed, %llu given", (unsigned long long)g.bytes, (unsigned long long)work_bytes);
         check_aligned(d_work, 16, "ae_points8_product_grad: work");
-        const unsigned groups = g.slices >= 192 ? 64 : g.slices >= 48 ? 16 : g.slices >= 8 ? 4 : 1;   // (the join's)
+        const unsigned groups = join_groups(g.slices);
         const uint64_t runs = m * (g.ldp / 4);
         if (g.tiles_m * g.tiles_k * g.slices > 0x3FFFFFull || runs * groups > 0xFFFF0000ull)
             fail(AE_ERR_INVALID_ARG, "ae_points8_product_grad: %llu rows are more than one call takes", (unsigned long long)m);

@@ -1,5 +1,6 @@
 // points8_plan.h -- which form of a kernel a size takes, and how many workgroups: the rules of the 8-bit store's calls, on the host and without HIP.
 #pragma once
+#include <algorithm>
 #include <cstdint>
 
 #include "../../include/annembed_hip.h"
@@ -39,7 +40,81 @@ inline BlocksPlan blocks_plan(uint64_t n, uint64_t dim, uint32_t type, bool look
     return p;
 }
 
+// ---- the product
+
+// 256 x 256 tiles read every operand least often but leave one workgroup on a CU: taken where they fill the chip several times and their edges waste
+// little (8192 x 16 384 x 4096 to bf16 779 against 915 us with 128 x 128, 8192^3 765 against 895, 8192 x 30 000 x 64 159 against 178; 1024 tiles of four blocks, 8192
+// x 8192 x 512, 78 against 82 and to f32 106 against 101; 4096 x 4096 x 1024, 256 tiles, 32.7 against 33.6 and to f32 40.3 either way; 4096 x 8192 x 256, 512 of
+// them, 27.8 against 25.4; 300 x 60 000 x 784, two rows of tiles for 300, 56 against 44).
+// Workgroups of 64 x 64 that split the coordinates, while each has a CU of its own, or nearly (170 x 258 x 1986 to bf16 9.4 against 19.4 us with 128 x 128 tiles; 1000 x
+// 1000 x 1000, 256 of them, 7.6 against 11.8; 128 x 12 000 x 784, 376, 11.4 against 11.8 and to f32 12.4 against 13.2; 512 x 4096 x 512, 512, 9.0 against 8.3
+// and 10.9 against 9.7).
+struct ProductPlan {
+    int tile;   // 64, 128 or 256 rows and points a workgroup
+    uint64_t tiles_m, tiles_n;
+};
+inline ProductPlan product_plan(uint64_t m, uint64_t n) {
+    auto tiles = [&](int tile) { return ProductPlan{tile, (m + tile - 1) / tile, (n + tile - 1) / tile}; };
+    const ProductPlan small = tiles(64), large = tiles(256);
+    if (small.tiles_m * small.tiles_n <= 384) return small;
+    if (large.tiles_m * large.tiles_n >= 1024 && large.tiles_m * 256 * 4 <= m * 5 && large.tiles_n * 256 * 4 <= n * 5) return large;
+    return tiles(128);
+}
+
+// Few rows: every workgroup quantises them itself, as the bf16 values they stand for in LDS.
+constexpr int kFew = 64;
+inline uint64_t few_lds_row(uint64_t dim) { return ((dim + kBlock - 1) / kBlock * kBlock) * 2 + 16; }   // (16 bytes more: neighbours start 4 banks apart)
+// 16 points a wave leave half of the chip's waves without work below 32 768 points: four waves share them then
+inline uint64_t few_points(uint64_t n, uint64_t dim) { return n >= 32768 || points8_blocks(dim) < 4 ? 64 : 16; }
+// One launch while the quantising that every workgroup does for itself, and the exact products, cost less than a launch does (one row against 5000 x 4000
+// 7.0 against 15.7 us, 16 against 3000 x 1400 9.1 against 10.3, but against 30 000 x 1400 33 against 18; 17 against 2000 x 300 6.1 against 8.2, 32
+// against 30 000 x 128 7.0 against 8.5, against 20 000 x 300 9.4 against 8.3; 48 against 20 000 x 28 9.1 against 8.2).
+inline bool few_rows(uint64_t m, uint64_t n, uint64_t dim) {
+    if (m > kFew || m * few_lds_row(dim) > 48 * 1024 || n >= 1ull << 30) return false;   // (64 points, 256 threads: fewer than 2^32)
+    const uint64_t tiles = m <= 16 ? 1 : m <= 32 ? 2 : 4, quantised = (n + few_points(n, dim) - 1) / few_points(n, dim) * m * dim;
+    return m <= 16 ? quantised <= 10000000 : tiles * 16 * n <= 1 << 20 && m * dim <= 10000 && quantised <= 2000000;
+}
+
 // ---- the gradient of the product
+
+constexpr int kStep = 64;    // points per step: 128 bytes of bf16
+
+struct GradPlan {
+    uint32_t fr;   // 64 rows of dc a tile, or 128
+    uint64_t tiles_m, tiles_k, slices, per_slice, ldp, bytes;
+};
+inline GradPlan grad_plan(uint64_t m, uint64_t n, uint64_t dim, uint32_t dctype) {
+    GradPlan best{};
+    const uint64_t steps = std::max<uint64_t>((n + kStep - 1) / kStep, 1), tiles_k = (dim + kBlock - 1) / kBlock, ldp = (dim + 3) / 4 * 4;
+    const uint64_t most = 0x3FFF0000ull / points8_row_bytes(dim) / kStep, least_slices = (steps + most - 1) / most;   // a slice's codes: less than 1 GiB
+    // What a choice costs, in us: a workgroup's beginning and end; its steps, with so many workgroups on a CU (measured at 300 x 60 000 x 784, between operands
+    // in cache and operands from memory; more workgroups do not fit or do not pay); the slices' sums, written and read again at 5 TB/s; the launch that
+    // joins them.  bf16, from memory: 300 x 60 000 x 784 56 us with 128 rows and two workgroups on a CU, 58 to 65 otherwise; 64 rows of it 22.4 with 64
+    // and one, 24 to 27 otherwise; 1000 x 1000 x 1000 in one slice 12.6 against 16 to 21 in several.
+    struct Choice { uint32_t fr, wgs; float step; };
+    static constexpr Choice bf16[] = {{1, 1, 0.43f}, {1, 2, 0.66f}, {2, 1, 0.55f}, {2, 2, 0.86f}};
+    static constexpr Choice f16[] = {{1, 1, 0.84f}, {1, 2, 1.1f}, {2, 1, 1.25f}, {2, 2, 1.76f}};
+    static constexpr Choice f32[] = {{1, 1, 1.07f}, {1, 2, 1.46f}};
+    const Choice* const choices = dctype == AE_TYPE_BF16 ? bf16 : dctype == AE_TYPE_F16 ? f16 : f32;
+    const int count = dctype == AE_TYPE_F32 ? 2 : 4;
+    double least = 0.;
+    for (int q = 0; q < count; q++) {
+        const Choice& c = choices[q];
+        const uint64_t tiles_m = (m + 64 * c.fr - 1) / (64 * c.fr), tiles = tiles_m * tiles_k, slots = 256 * c.wgs;
+        for (const uint64_t want : {(uint64_t)1, slots / tiles}) {
+            const uint64_t slices = std::max<uint64_t>({1, least_slices, std::min(want, (steps + 3) / 4)}), per = (steps + slices - 1) / slices, used = (steps + per - 1) / per;
+            const double rounds = (double)((tiles * used + slots - 1) / slots);
+            const double cost = rounds * ((c.fr == 1 ? 2 : 5) + per * c.step) + (used > 1 ? 4. + used * (0.005 + m * ldp * 8 / 5.1e6) : 0.);
+            if (best.fr && cost >= least) continue;
+            least = cost;
+            best = GradPlan{c.fr, tiles_m, tiles_k, used, per * kStep, ldp, used > 1 ? used * m * ldp * 4 : 0};
+        }
+    }
+    return best;
+}
+
+// groups of threads that share a run of the slices' sums when they are joined
+inline unsigned join_groups(uint64_t slices) { return slices >= 192 ? 64 : slices >= 48 ? 16 : slices >= 8 ? 4 : 1; }
 
 // bytes of dc from a tile's first value to its last one in a slice of the points, and not one more: what a 16-byte piece has behind them is not fetched
 constexpr uint32_t grad_range(uint32_t rows, uint32_t row_bytes, uint32_t points, uint32_t size) { return (rows - 1) * row_bytes + points * size; }

@@ -7,8 +7,6 @@
 // type and however many rows there are.
 #include "points8.h"
 
-#include <algorithm>
-
 using namespace ae;
 
 namespace {
@@ -372,12 +370,12 @@ __global__ void __launch_bounds__(256, 2) product_deep_kernel(ProductArgs a) {
 }
 
 template <int BM, int BN, int WM>
-void launch_tiles(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t ctype, uint64_t ldc, hipStream_t s) {
-    const uint64_t tiles_m = (x.rows + BM - 1) / BM, tiles_n = (p.rows + BN - 1) / BN, tiles = tiles_m * tiles_n;
+void launch_tiles(const Rows8& x, const Rows8& p, const ProductPlan& plan, uint64_t dim, void* d_c, uint32_t ctype, uint64_t ldc, hipStream_t s) {
+    const uint64_t tiles = plan.tiles_m * plan.tiles_n;
     if (tiles > 0x3FFFFFFFull) fail(AE_ERR_INVALID_ARG, "ae_points8_product: %llu x %llu are more products than one call takes", (unsigned long long)x.rows, (unsigned long long)p.rows);
     constexpr unsigned threads = (BM / WM) * (BN / 64) * 64, bytes = 2 * (BM + BN) * kBlock, resident = 256 * (bytes > 80 * 1024 ? 1 : 2);
     const bool near = ldc * type_size(ctype) < 0x7FFF0000ull / BM;
-    const ProductArgs a{x, p, points8_blocks(dim), d_c, ldc, (uint32_t)tiles_m, (uint32_t)tiles_n, near ? 1u : 0u};
+    const ProductArgs a{x, p, points8_blocks(dim), d_c, ldc, (uint32_t)plan.tiles_m, (uint32_t)plan.tiles_n, near ? 1u : 0u};
     const unsigned grid = tiles < resident ? (unsigned)((tiles + 7) / 8 * 8) : resident;
     by_type(ctype, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
@@ -386,45 +384,24 @@ void launch_tiles(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint3
     check_launch("points8_product");
 }
 
-// 256 x 256 tiles read every operand least often but leave one workgroup on a CU: taken where they fill the chip several times and their edges waste
-// little (8192 x 16 384 x 4096 to bf16 779 against 915 us with 128 x 128, 8192^3 765 against 895, 8192 x 30 000 x 64 159 against 178; 1024 tiles of four blocks, 8192
-// x 8192 x 512, 78 against 82 and to f32 106 against 101; 4096 x 4096 x 1024, 256 tiles, 32.7 against 33.6 and to f32 40.3 either way; 4096 x 8192 x 256, 512 of
-// them, 27.8 against 25.4; 300 x 60 000 x 784, two rows of tiles for 300, 56 against 44).
 void product(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t ctype, uint64_t ldc, hipStream_t s) {
-    // Workgroups of 64 x 64 that split the coordinates, while each has a CU of its own, or nearly (170 x 258 x 1986 to bf16 9.4 against 19.4 us with 128 x 128 tiles; 1000 x
-    // 1000 x 1000, 256 of them, 7.6 against 11.8; 128 x 12 000 x 784, 376, 11.4 against 11.8 and to f32 12.4 against 13.2; 512 x 4096 x 512, 512, 9.0 against 8.3
-    // and 10.9 against 9.7).
-    const uint64_t deep_m = (x.rows + 63) / 64, deep_n = (p.rows + 63) / 64;
-    if (deep_m * deep_n <= 384) {
-        const ProductArgs a{x, p, points8_blocks(dim), d_c, ldc, (uint32_t)deep_m, (uint32_t)deep_n, 0};
+    const ProductPlan plan = product_plan(x.rows, p.rows);
+    if (plan.tile == 64) {
+        const ProductArgs a{x, p, points8_blocks(dim), d_c, ldc, (uint32_t)plan.tiles_m, (uint32_t)plan.tiles_n, 0};
         by_type(ctype, [&](auto ty) {
             constexpr int TYPE = decltype(ty)::value;
-            hipLaunchKernelGGL((product_deep_kernel<TYPE>), dim3((unsigned)(deep_m * deep_n)), dim3(256), 4 * 16 * 64 * 16, s, a);
+            hipLaunchKernelGGL((product_deep_kernel<TYPE>), dim3((unsigned)(plan.tiles_m * plan.tiles_n)), dim3(256), 4 * 16 * 64 * 16, s, a);
         });
         check_launch("points8_product_deep");
         return;
     }
-    const uint64_t tm = (x.rows + 255) / 256, tn = (p.rows + 255) / 256;
-    if (tm * tn >= 1024 && tm * 256 * 4 <= x.rows * 5 && tn * 256 * 4 <= p.rows * 5) launch_tiles<256, 256, 128>(x, p, dim, d_c, ctype, ldc, s);
-    else launch_tiles<128, 128, 64>(x, p, dim, d_c, ctype, ldc, s);
+    if (plan.tile == 256) launch_tiles<256, 256, 128>(x, p, plan, dim, d_c, ctype, ldc, s);
+    else launch_tiles<128, 128, 64>(x, p, plan, dim, d_c, ctype, ldc, s);
 }
 
 // Few rows: bound by the points' bytes, which go from memory straight to the matrix cores (16 points a wave, 32 coordinates of a block
 // a lane).  Every workgroup quantises the rows itself, into LDS as the bf16 values they stand for, while its first points are on their way: one
 // launch.  SPLIT waves share the blocks of a group of points where there are few points.
-constexpr int kFew = 64;
-constexpr uint64_t few_lds_row(uint64_t dim) { return ((dim + kBlock - 1) / kBlock * kBlock) * 2 + 16; }   // (16 bytes more: neighbours start 4 banks apart)
-// 16 points a wave leave half of the chip's waves without work below 32 768 points: four waves share them then
-uint64_t few_points(uint64_t n, uint64_t dim) { return n >= 32768 || points8_blocks(dim) < 4 ? 64 : 16; }
-// One launch while the quantising that every workgroup does for itself, and the exact products, cost less than a launch does (one row against 5000 x 4000
-// 7.0 against 15.7 us, 16 against 3000 x 1400 9.1 against 10.3, but against 30 000 x 1400 33 against 18; 17 against 2000 x 300 6.1 against 8.2, 32
-// against 30 000 x 128 7.0 against 8.5, against 20 000 x 300 9.4 against 8.3; 48 against 20 000 x 28 9.1 against 8.2).
-bool few_rows(uint64_t m, uint64_t n, uint64_t dim) {
-    if (m > kFew || m * few_lds_row(dim) > 48 * 1024 || n >= 1ull << 30) return false;   // (64 points, 256 threads: fewer than 2^32)
-    const uint64_t tiles = m <= 16 ? 1 : m <= 32 ? 2 : 4, quantised = (n + few_points(n, dim) - 1) / few_points(n, dim) * m * dim;
-    return m <= 16 ? quantised <= 10000000 : tiles * 16 * n <= 1 << 20 && m * dim <= 10000 && quantised <= 2000000;
-}
-
 template <int XTYPE, int SPLIT, int TILES>   // TILES of 16 rows
 __global__ void __launch_bounds__(256) product_few_kernel(const typename Elem<XTYPE>::T* __restrict__ x, uint32_t m, uint64_t ldx, uint32_t dim, Rows8 p, void* c_, uint32_t ctype, uint64_t ldc) {
     constexpr int GROUPS = 4 / SPLIT, AHEAD = 4;   // groups of 16 points a workgroup; blocks whose codes are fetched together

@@ -5,6 +5,9 @@ import subprocess
 
 import pytest
 
+from tests.test_gpu_points8_forms import GRADIENTS
+from tests.test_gpu_points8_sums import SHAPES
+
 ROOT = pathlib.Path(__file__).resolve().parent.parent
 F32, BF16, F16 = range(3)
 PROGRAM = r"""
@@ -24,6 +27,12 @@ int main() {
             printf("%d %u %d\n", p.trips, p.grid, (int)write_looks(a[0], a[1]));
         } else if (!strcmp(what, "range")) {   // rows lddc points size
             printf("%u\n", grad_range((uint32_t)a[0], (uint32_t)(a[1] * a[3]), (uint32_t)a[2], (uint32_t)a[3]));
+        } else if (!strcmp(what, "product")) {   // m n dim: whether rows are few, points a workgroup takes then, the tile otherwise, tiles
+            const ProductPlan p = product_plan(a[0], a[1]);
+            printf("%d %d %d %llu\n", (int)few_rows(a[0], a[1], a[2]), (int)few_points(a[1], a[2]), p.tile, (unsigned long long)(p.tiles_m * p.tiles_n));
+        } else if (!strcmp(what, "gradient")) {   // m n dim type
+            const GradPlan p = grad_plan(a[0], a[1], a[2], (uint32_t)a[3]);
+            printf("%u %llu %llu %u %llu\n", p.fr * 64, (unsigned long long)p.slices, (unsigned long long)p.per_slice, p.slices > 1 ? join_groups(p.slices) : 0, (unsigned long long)p.bytes);
         } else return 2;
     }
 }
@@ -67,3 +76,42 @@ def test_the_gradient_reads_nothing_behind_its_tensor(plan):
     """a tile's buffer ends with its last row's last value, whether that is a whole dword or the first half of one"""
     for rows, lddc, points, size in ((1, 1, 1, 2), (1, 129, 129, 2), (64, 129, 129, 2), (128, 60001, 60001, 2), (5, 140, 129, 2), (64, 7, 7, 4), (3, 64, 64, 2)):
         assert plan("range", rows, lddc, points, size)[0] == ((rows - 1) * lddc + points) * size
+
+
+def test_the_products_that_are_tested_take_every_form(plan):
+    """few rows in 1, 2 and 4 tiles of 16, groups of points whole and shared; 64 x 64, 128 x 128 and 256 x 256 tiles"""
+    forms = set()
+    for m, n, dim in SHAPES:
+        few, points, tile, _ = plan("product", m, n, dim)
+        forms.add(("few", 1 if m <= 16 else 2 if m <= 32 else 4, points) if few else tile)
+        forms.add(tile)   # (of another store's points: never few)
+    assert forms == {("few", 1, 64), ("few", 1, 16), ("few", 2, 64), ("few", 2, 16), ("few", 4, 64), 64, 128, 256}
+
+
+def test_the_borders_of_the_products_forms(plan):
+    assert plan("product", 64 * 16, 64 * 24, 100)[2:] == (64, 384) and plan("product", 64 * 16, 64 * 24 + 1, 100)[2] == 128
+    assert plan("product", 256 * 32, 256 * 32, 100)[2:] == (256, 1024) and plan("product", 256 * 32, 256 * 31, 100)[2] == 128 and plan("product", 300, 256 * 600, 100)[2] == 128
+    assert plan("product", 16, 32768, 784)[0] == 1 and plan("product", 65, 100, 28)[0] == 0 and plan("product", 64, 16384, 28)[0] == 1 and plan("product", 64, 16385, 28)[0] == 0
+    for n in (1 << 30, (1 << 32) - 2):
+        assert plan("product", 1, n, 1)[0] == 0
+
+
+def test_the_gradients_that_are_tested_take_every_form(plan):
+    forms, joins = set(), set()
+    for m, n, dim in GRADIENTS:
+        for kind in (F32, BF16, F16):
+            rows, slices, per, groups, _ = plan("gradient", m, n, dim, kind)
+            assert (slices - 1) * per < n <= slices * per and per % 64 == 0
+            forms.add((kind, rows, slices > 1))
+            joins.add(groups)
+    assert forms == {(kind, rows, more) for kind in (F32, BF16, F16) for rows in (64, 128) for more in (False, True)} - {(F32, 128, False), (F32, 128, True)}
+    assert joins == {0, 1, 4, 16, 64}
+
+
+def test_scratch_of_the_gradient(plan):
+    """the sums of all slices, rows of whole 16 bytes; none where one slice writes the result itself"""
+    for m, n, dim in GRADIENTS + [(1, 1, 1), (1 << 20, 70, 3), (3, 1 << 26, 1 << 20)]:
+        for kind in (F32, BF16, F16):
+            rows, slices, per, _, size = plan("gradient", m, n, dim, kind)
+            assert size == (slices * m * (-(-dim // 4) * 4) * 4 if slices > 1 else 0)
+            assert per * (-(-dim // 16) * 16) <= 0x3FFF0000   # a slice's codes: 32-bit offsets reach them
