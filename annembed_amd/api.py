@@ -200,7 +200,8 @@ class KGraph(_Handle):
 
     @classmethod
     def bruteforce_l2_points8(cls, points, nbng, n=None, first=0):
-        """the exact graph of points first ... first + n - 1 of a Points8 store, as it holds them (ae_kgraph_bruteforce_l2_points8)"""
+        """the exact graph of points first ... first + n - 1 of a Points8 store, as it holds them (ae_kgraph_bruteforce_l2_points8);
+        takes n * dim * 4 bytes of device memory while it runs, refuses points with a NaN coordinate"""
         import torch
         n, first = points._range(n, first)
         h = C.c_void_p()

@@ -100,7 +100,8 @@ __device__ __forceinline__ bool place_of(const GradArgs& a, uint32_t& slice, uin
 // the rows and all coordinates, so each value of dc is split once.  dc goes to LDS as it is, three steps deep.  (Straight to the lanes that
 // multiply it, 16 bytes of 16 rows each, every lane would be an access of its own to the cache.)  The codes are turned on the way to LDS: a thread takes
 // 4 coordinates of 8 points, widens them under the products of the step before and writes 8 points of one coordinate as 16 bytes.  One
-// barrier a step.  8192 x 8192 x 4096 of f32: 970 TF of the three partial products, at the rate of the matrix cores; 300 x 60 000 x 784: 107 us.
+// barrier a step.  8192 x 8192 x 4096 of f32: 970 TF of the three partial products (of the 1413 that a large bf16 product of the library reaches); 300 x
+// 60 000 x 784: 107 us.  What it waits for is LDS: every wave splits the values it takes, and 112 KB move for 128 x 128 x 64.
 template <int TYPE, int FR> constexpr int grad_lds() { return 3 * 64 * FR * kStep * (TYPE == AE_TYPE_F32 ? 4 : 2) + 2 * kBlock * 128; }   // 56 or 80 KB: two workgroups a CU
 
 template <int TYPE, int FR, bool VEC>   // VEC: the copies' 32-bit offsets do for dc
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(256, 2) grad_tile_kernel(GradArgs a) {
 // in a fragment, so the codes are widened in the registers they are used from, and each wave reads all rows of dc: LDS moves 48 KB for
 // 128 x 128 x 64 where the kernel above moves 112 (300 x 60 000 x 784: 47 us against 52, 4096 x 32 768 x 1024: 256 against 303, 1075 TF of the 1413 that a
 // large bf16 product of the library reaches).  dc and the codes come by copies to LDS three deep; the codes are read two steps ahead and widened under
-// the products, whose waits for one another and for the barrier of a step are what bounds it: the matrix cores are busy for 45 % of the time.
+// the products, whose waits for one another and for the barrier of a step are what bounds it: the matrix cores are busy for 30 % of the time at 300 x 60 000 x 784.
 constexpr int kTurnStage = kStep * 128;   // codes of a step
 template <int FR> constexpr int turn_lds() { return 3 * (16 * FR * kStep * 2 + kTurnStage + 1024); }   // 51 or 75 KB for 64 or 128 rows
 

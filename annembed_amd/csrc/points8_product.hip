@@ -76,6 +76,8 @@ struct Walk {
 // The blocks of all tiles of a workgroup form one stream: the copy runs two blocks ahead of the products, across the end of a tile, and the
 // stores of a tile drain under the next one.  A step's fragment is read two steps ahead.  Two steps before its end a block's stage has been read by
 // everybody and the next one has to be there: one barrier a block.  The loop's body has no branch (copies beyond the last tile fetch nothing).
+// 8192 x 16 384 x 4096 to bf16 779 us in 256 x 256 tiles, 1411 TF, what a large bf16 product of the library reaches (their sums fill the registers: 20 of 256 spill, to
+// f32 42); 300 x 60 000 x 784 44 us in 128 x 128, where the matrix cores are busy for 31 % of the time: 28 % of the rows are padding, a tile has 7 blocks.
 template <int TYPE, int BM, int BN, int WM>
 __global__ void __launch_bounds__((BM / WM) * (BN / 64) * 64, (BM + BN) * kBlock * 2 > 80 * 1024 ? (BM / WM) * (BN / 64) / 4 : (BM / WM) * (BN / 64) / 2)
 product_tile_kernel(ProductArgs a) {

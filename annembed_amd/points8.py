@@ -1,6 +1,6 @@
 """Points held in 8 bits, the product of rows with them and its gradient, and the teacher's loss, on torch tensors.
 
-Beside the graph and the embedding (no counterpart in the reference): a bank of points too large for 32 bits, an encoder trained so that the
+Beside the graph and the embedding (no counterpart in the reference): a bank of points in a quarter of f32's memory, an encoder trained so that the
 softmax of its scores against the bank follows the graph's edge probabilities.
 
     bank = Points8(capacity=n, dim=784)
