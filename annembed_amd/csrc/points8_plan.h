@@ -42,10 +42,11 @@ inline BlocksPlan blocks_plan(uint64_t n, uint64_t dim, uint32_t type, bool look
 
 // ---- the product
 
-// 256 x 256 tiles read every operand least often but leave one workgroup on a CU: taken where they fill the chip several times and their edges waste
-// little (8192 x 16 384 x 4096 to bf16 779 against 915 us with 128 x 128, 8192^3 765 against 895, 8192 x 30 000 x 64 159 against 178; 1024 tiles of four blocks, 8192
-// x 8192 x 512, 78 against 82 and to f32 106 against 101; 4096 x 4096 x 1024, 256 tiles, 32.7 against 33.6 and to f32 40.3 either way; 4096 x 8192 x 256, 512 of
-// them, 27.8 against 25.4; 300 x 60 000 x 784, two rows of tiles for 300, 56 against 44).
+// 256 x 256 tiles read every operand least often but leave one workgroup on a CU: taken where a tile has 8 blocks or more, whole rounds of tiles fill the chip to 7 / 8 and
+// edges waste little.  To bf16, against 128 x 128: 8192 x 16 384 x 4096 779 and 915 us, 4096 x 8192 x 4096 203 and 233, 4096 x 4096 x 4096 99 and 117, 8192 x 8192 x 1024 121 and
+// 134, 3840 x 4096 x 2048, 240 tiles, 53 and 60 (to f32 62 and 64); but 8192 x 8192 x 512 77 and 81 (to f32 107 and 100), 8192 x 16 384 x 128 87 and 72, 6144 x 6144 x
+// 4096, 576 tiles, 282 and 259, 300 x 60 000 x 784, two rows of tiles for 300, 56 and 44.  (Few blocks and very many tiles can go either way: 8192 x 30 000 x 64 159 and 178, 16 384 x
+// 16 384 x 128 154 and 138.)
 // Workgroups of 64 x 64 that split the coordinates, while each has a CU of its own, or nearly (170 x 258 x 1986 to bf16 9.4 against 19.4 us with 128 x 128 tiles; 1000 x
 // 1000 x 1000, 256 of them, 7.6 against 11.8; 128 x 12 000 x 784, 376, 11.4 against 11.8 and to f32 12.4 against 13.2; 512 x 4096 x 512, 512, 9.0 against 8.3
 // and 10.9 against 9.7).
@@ -53,11 +54,12 @@ struct ProductPlan {
     int tile;   // 64, 128 or 256 rows and points a workgroup
     uint64_t tiles_m, tiles_n;
 };
-inline ProductPlan product_plan(uint64_t m, uint64_t n) {
+inline ProductPlan product_plan(uint64_t m, uint64_t n, uint64_t dim) {
     auto tiles = [&](int tile) { return ProductPlan{tile, (m + tile - 1) / tile, (n + tile - 1) / tile}; };
     const ProductPlan small = tiles(64), large = tiles(256);
     if (small.tiles_m * small.tiles_n <= 384) return small;
-    if (large.tiles_m * large.tiles_n >= 1024 && large.tiles_m * 256 * 4 <= m * 5 && large.tiles_n * 256 * 4 <= n * 5) return large;
+    const uint64_t count = large.tiles_m * large.tiles_n, rounds = (count + 255) / 256;
+    if (points8_blocks(dim) >= 8 && count * 8 >= rounds * 256 * 7 && large.tiles_m * 256 * 4 <= m * 5 && large.tiles_n * 256 * 4 <= n * 5) return large;
     return tiles(128);
 }
 

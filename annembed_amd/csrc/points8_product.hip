@@ -387,7 +387,7 @@ void launch_tiles(const Rows8& x, const Rows8& p, const ProductPlan& plan, uint6
 }
 
 void product(const Rows8& x, const Rows8& p, uint64_t dim, void* d_c, uint32_t ctype, uint64_t ldc, hipStream_t s) {
-    const ProductPlan plan = product_plan(x.rows, p.rows);
+    const ProductPlan plan = product_plan(x.rows, p.rows, dim);
     if (plan.tile == 64) {
         const ProductArgs a{x, p, points8_blocks(dim), d_c, ldc, (uint32_t)plan.tiles_m, (uint32_t)plan.tiles_n, 0};
         by_type(ctype, [&](auto ty) {

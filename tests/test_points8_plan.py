@@ -28,7 +28,7 @@ int main() {
         } else if (!strcmp(what, "range")) {   // rows lddc points size
             printf("%u\n", grad_range((uint32_t)a[0], (uint32_t)(a[1] * a[3]), (uint32_t)a[2], (uint32_t)a[3]));
         } else if (!strcmp(what, "product")) {   // m n dim: whether rows are few, points a workgroup takes then, the tile otherwise, tiles
-            const ProductPlan p = product_plan(a[0], a[1]);
+            const ProductPlan p = product_plan(a[0], a[1], a[2]);
             printf("%d %d %d %llu\n", (int)few_rows(a[0], a[1], a[2]), (int)few_points(a[1], a[2]), p.tile, (unsigned long long)(p.tiles_m * p.tiles_n));
         } else if (!strcmp(what, "gradient")) {   // m n dim type
             const GradPlan p = grad_plan(a[0], a[1], a[2], (uint32_t)a[3]);
@@ -90,7 +90,9 @@ def test_the_products_that_are_tested_take_every_form(plan):
 
 def test_the_borders_of_the_products_forms(plan):
     assert plan("product", 64 * 16, 64 * 24, 100)[2:] == (64, 384) and plan("product", 64 * 16, 64 * 24 + 1, 100)[2] == 128
-    assert plan("product", 256 * 32, 256 * 32, 100)[2:] == (256, 1024) and plan("product", 256 * 32, 256 * 31, 100)[2] == 128 and plan("product", 300, 256 * 600, 100)[2] == 128
+    for m, n, dim, tile in ((4096, 4096, 897, 256), (4096, 4096, 896, 128), (4096, 3584, 2000, 256), (4096, 3328, 2000, 128), (4097, 4096, 2000, 128), (8192, 8192, 1024, 256),
+                            (8192, 7936, 1024, 256), (300, 256 * 600, 2000, 128)):
+        assert plan("product", m, n, dim)[2] == tile
     assert plan("product", 16, 32768, 784)[0] == 1 and plan("product", 65, 100, 28)[0] == 0 and plan("product", 64, 16384, 28)[0] == 1 and plan("product", 64, 16385, 28)[0] == 0
     for n in (1 << 30, (1 << 32) - 2):
         assert plan("product", 1, n, 1)[0] == 0
