@@ -5,6 +5,7 @@ Embedder / DiffusionMaps / SvdApprox) over the C ABI of libannembed_hip.so.  All
 (hand-written HIP kernels; rocPRIM sort / scan as primitives beside them); there is no CPU fallback: importing the API without the built library, or
 calling it without a GPU, fails loudly.
 """
+import sys as _sys
 from importlib.util import find_spec as _find_spec
 
 from ._lib import (AE_CE_AUTO, AE_CE_EVENT, AE_CE_HOGWILD, AE_CE_ORDERED, AE_CE_SAMPLE_RACY, AE_CE_SEQUENTIAL, AE_CE_SLICED, AE_PRECISION_F32, AE_PRECISION_F64, AE_SAMPLER_ALIAS, AE_SAMPLER_ROWCDF, AnnembedError, LIB_PATH,  # noqa: F401
@@ -29,5 +30,5 @@ __all__ = [
     "adaptative_range_finder_matrep",
     "set_summation_order", "AnnembedError", "load",
 ]
-if _find_spec("torch") is not None:   # (looks for it, does not import it)
+if (_sys.modules["torch"] if "torch" in _sys.modules else _find_spec("torch")) is not None:   # (looks for it, does not import it)
     __all__ += ["Points8", "teacher_loss", "teacher_grad"]

@@ -21,3 +21,9 @@ def test_all_names_without_torch():
 def test_all_names_with_torch():
     r = run("from annembed_amd import *\nassert Points8 and teacher_loss and teacher_grad and KGraph")
     assert r.returncode == 0, r.stderr
+
+
+def test_all_names_with_a_torch_that_nobody_found():
+    """a module put into sys.modules by hand has no spec"""
+    r = run("import sys, types; sys.modules['torch'] = types.ModuleType('torch')\nimport annembed_amd as A\nassert 'Points8' in A.__all__ and A.KGraph")
+    assert r.returncode == 0, r.stderr
