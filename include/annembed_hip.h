@@ -602,9 +602,10 @@ int32_t ae_embedder_get_quality_estimate_from_edge_length(const ae_embedder *e, 
  *
  * Format: a row of `dim` coordinates in blocks of 128 (the last may be shorter).  a = the largest magnitude among the finite values of the
  * block, e = the smallest integer >= -126 with a <= 448 * 2^e.  A coordinate is the e4m3 number nearest to x * 2^-e (ties to even) whose value
- * f32 has: where e = 120 the largest is 240, and magnitudes from 248 * 2^120 on are held as 240 * 2^120; NaN and the infinities are held as NaN.  The scale byte of the block is e + 127.  The value held is code * 2^e.  The scale is a power of two
- * because that costs an 8-bit float none of its relative precision (2^-4), makes x * 2^-e exact (the codes do not depend on how the
- * division is done) and the value held exact in bf16, which the matrix cores multiply.
+ * f32 has: where e = 120 the largest is 240, and magnitudes from 248 * 2^120 on are held as 240 * 2^120; NaN and the infinities are held as
+ * NaN.  The scale byte of the block is e + 127.  The value held is code * 2^e.  The scale is a power of two because that costs an 8-bit float
+ * none of its relative precision (2^-4), makes x * 2^-e exact (the codes do not depend on how the division is done) and the value held exact
+ * in bf16, which the matrix cores multiply.
  * ------------------------------------------------------------------------------------------------ */
 enum { AE_TYPE_F32 = 0, AE_TYPE_BF16 = 1, AE_TYPE_F16 = 2 };
 typedef struct ae_points8 ae_points8;
@@ -650,8 +651,8 @@ int32_t ae_kgraph_bruteforce_l2_points8(const ae_points8 *p, uint64_t first, uin
      AE_TEACHER_LOGITS  the teacher's logit t_j: p = softmax(t / temperature) over the row's list (-inf: p = 0).
    With ln q = ln softmax(s / temperature):   loss_r = w_r sum_j p_j (ln p_j - ln q_{idx_j}),   w_r = d_row_weight[r] (NULL: 1)
                                                d loss_r / d s_v = w_r (q_v sum_j p_j - sum_{j: idx_j = v} p_j) / temperature.
-   The temperature is positive, finite and not denormal.  A column may come several times in a list: its probabilities add up.  p_j = 0 contributes nothing; p_j > 0 on a logit of -inf makes the
-   loss +inf.  A row of weight 0 is not looked at (its logits and list may hold anything): loss 0, gradient 0; so are rows whose logits
+   The temperature is positive, finite and not denormal.  A column may come several times in a list: its probabilities add up.  p_j = 0
+   contributes nothing; p_j > 0 on a logit of -inf makes the loss +inf.  A row of weight 0 is not looked at (its logits and list may hold anything): loss 0, gradient 0; so are rows whose logits
    are all -inf.  A column index >= cols, a NaN or a +inf among a row's logits makes that row NaN.
    d_loss[rows] f32; d_stats[rows][2] f32: (the largest logit, ln sum_v exp((s_v - largest) / temperature)), (-inf, 0) for rows left out --
    what ae_teacher_grad needs.  d_grad (NULL: not wanted): the gradient of sum_r loss_r in the logits' type, in the same pass; it may be
