@@ -142,3 +142,20 @@ def test_captured_scattered_writes(A, n, dim):
             store.write(x[:100] * 2, first=turn)
             store.write(x.flip(0), slots=slots)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_product_of_rows_far_apart(A, dtype):
+    """rows of the result farther apart than the 32-bit offsets of a 128 x 128 tile's stores reach, with a rest of both; nothing between them is written"""
+    m, n, dim = 130, 8333, 200
+    rng = np.random.default_rng(m)
+    p, x = integers(rng, 7, n, dim), integers(rng, 7, m, dim)
+    bank = A.Points8(n, dim)
+    bank.write(torch.from_numpy(p).cuda())
+    step = 8_400_001 if dtype != torch.float32 else 4_200_001
+    room = torch.full(((m - 1) * step + n,), 7.0, dtype=dtype, device="cuda")
+    far = room.as_strided((m, n), (step, 1))
+    for turn in range(2):   # (tiles follow one another in a workgroup: the second call's find the first's results)
+        bank.product(torch.from_numpy(x).cuda(), out=far)
+        assert torch.equal(far.cpu(), torch.from_numpy(x @ p.T).to(dtype))
+    assert (room.as_strided((m - 1, step - n), (step, 1), n) == 7).all()

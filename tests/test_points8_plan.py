@@ -117,3 +117,7 @@ def test_scratch_of_the_gradient(plan):
             rows, slices, per, _, size = plan("gradient", m, n, dim, kind)
             assert size == (slices * m * (-(-dim // 4) * 4) * 4 if slices > 1 else 0)
             assert per * (-(-dim // 16) * 16) <= 0x3FFF0000   # a slice's codes: 32-bit offsets reach them
+
+
+def test_the_product_of_rows_far_apart_takes_tiles_of_128(plan):
+    assert plan("product", 130, 8333, 200)[0] == 0 and plan("product", 130, 8333, 200)[2] == 128
