@@ -57,7 +57,7 @@ struct Walk {
     __device__ __forceinline__ bool here() const { return at < count; }
     __device__ __forceinline__ void tile(uint32_t& tm, uint32_t& tn) const {
         const uint32_t id = first + at, panel = id / (kPanel * tiles_n), in = id - panel * kPanel * tiles_n;
-        const uint32_t rows = min(kPanel, tiles_m - panel * kPanel);
+        const uint32_t rows = max(1u, min(kPanel, tiles_m - panel * kPanel));   // (past the last tile there is no panel: nobody uses what comes out, but 0 does not divide)
         tn = in / rows;
         tm = panel * kPanel + in - tn * rows;
     }
